@@ -51,6 +51,9 @@ EXPORTED_SYMBOLS = (
     "bevk_ms_deform_attn_forward",
     "bevk_ms_deform_attn_backward_workspace_bytes",
     "bevk_ms_deform_attn_backward",
+    "bevk_group_norm_act_workspace_bytes",
+    "bevk_group_norm_act_forward",
+    "bevk_group_norm_act_backward",
 )
 
 
@@ -107,6 +110,24 @@ class DcnBackwardDataArgs(ctypes.Structure):
         ("grad_input_strides", ctypes.c_int64 * 4),
         ("grad_offset_strides", ctypes.c_int64 * 4),
         ("grad_mask_strides", ctypes.c_int64 * 4),
+    ]
+
+
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+
+
+class GroupNormProblem(ctypes.Structure):
+    """Mirror of ``bevk_group_norm_problem``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("param_dtype", ctypes.c_int),
+        ("batch", ctypes.c_int), ("channels", ctypes.c_int), ("groups", ctypes.c_int),
+        ("act", ctypes.c_int),
+        ("pixels", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("input_strides", ctypes.c_int64 * 2),
+        ("output_strides", ctypes.c_int64 * 2),
+        ("grad_output_strides", ctypes.c_int64 * 2),
     ]
 
 
@@ -176,6 +197,13 @@ def lib():
     L.bevk_ms_deform_attn_backward.restype = i
     L.bevk_ms_deform_attn_backward.argtypes = ([vp, i64p, i64p, vp, vp, vp] + [i] * 8 +
                                                [vp, vp, vp, vp, ctypes.c_size_t, i, vp])
+    gp = ctypes.POINTER(GroupNormProblem)
+    L.bevk_group_norm_act_workspace_bytes.restype = sz
+    L.bevk_group_norm_act_workspace_bytes.argtypes = [gp, i]
+    L.bevk_group_norm_act_forward.restype = i
+    L.bevk_group_norm_act_forward.argtypes = [gp] + [vp] * 7 + [sz, vp]
+    L.bevk_group_norm_act_backward.restype = i
+    L.bevk_group_norm_act_backward.argtypes = [gp] + [vp] * 10 + [sz, vp]
     _lib = L
     return L
 

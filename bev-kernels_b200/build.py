@@ -5,8 +5,8 @@
 1. ``libbevk.so``: every ``csrc/*.cu`` compiled by nvcc for sm_100a only
    (``-gencode arch=compute_100a,code=sm_100a``), exporting the C ABI of
    ``include/bevk.h``.
-2. The torch extensions ``_modulated_deform_conv_ext`` and ``_ms_deform_attn_ext``
-   (thin C++ layers over the C ABI; no CUDA code of their own), built with
+2. The torch extensions ``_modulated_deform_conv_ext``, ``_ms_deform_attn_ext`` and
+   ``_bevk_train_ext`` (thin C++ layers over the C ABI; no CUDA code of their own), built with
    ``setup.py build_ext --inplace`` next to this file.
 
 Outputs stay inside this directory so they travel with the source tree.
@@ -74,7 +74,8 @@ def build_lib(verbose: bool = False, extra_flags=()) -> str:
 def build_torch_ext(verbose: bool = False) -> None:
     srcs = glob.glob(os.path.join(CSRC, "torch_ext_*.cpp"))
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
-    outs = [os.path.join(HERE, n + suffix) for n in ("_modulated_deform_conv_ext", "_ms_deform_attn_ext")]
+    outs = [os.path.join(HERE, n + suffix) for n in (
+        "_modulated_deform_conv_ext", "_ms_deform_attn_ext", "_bevk_train_ext")]
     deps = srcs + [LIB, os.path.join(INCLUDE, "bevk.h"), os.path.join(HERE, "setup.py")]
     if not any(_stale(o, deps) for o in outs):
         return

@@ -144,6 +144,16 @@ int launch_dcn_im2col(const bevk_dcn_problem *p, const DcnDims &d, const void *x
                       const void *off, const void *msk, void *col, int col_layout,
                       cudaStream_t stream);
 
+// Group norm with activation (group_norm.cu).
+size_t group_norm_workspace_bytes(const bevk_group_norm_problem *q, bool backward);
+int launch_group_norm_forward(const bevk_group_norm_problem *q, const void *x, const void *w,
+                              const void *b, void *y, float *mean, float *rstd, void *ws,
+                              size_t ws_bytes, cudaStream_t stream);
+int launch_group_norm_backward(const bevk_group_norm_problem *q, const void *dy, const void *x,
+                               const float *mean, const float *rstd, const void *w, const void *b,
+                               void *dx, void *dw, void *db, void *ws, size_t ws_bytes,
+                               cudaStream_t stream);
+
 // Device watchdog word (one per device, defined in dcn_tc.cu).
 int read_and_clear_watchdog(int device, unsigned int *code);
 // Limit of the fused DCN kernel's pipeline barrier waits on `device` (0: the

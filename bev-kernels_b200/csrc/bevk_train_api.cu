@@ -1,0 +1,115 @@
+// bevk_train_api.cu -- the extern "C" entry points of the training-side
+// operators declared in include/bevk.h: argument validation and dispatch.  No
+// entry point allocates device memory.
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "bevk.h"
+#include "bevk_internal.h"
+
+using namespace bevk;
+
+namespace {
+
+bool known_dtype(int dtype) {
+  return dtype == BEVK_DTYPE_F32 || dtype == BEVK_DTYPE_F16 || dtype == BEVK_DTYPE_BF16;
+}
+
+// Checks a group norm problem; `backward` also looks at grad_output's strides.
+int check_group_norm(const bevk_group_norm_problem *p, bool backward) {
+  if (!p) return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act: null problem");
+  if (!known_dtype(p->dtype))
+    return fail(BEVK_ERR_UNSUPPORTED, "group_norm_act: dtype %d (f32, f16, bf16)", p->dtype);
+  if (p->param_dtype != p->dtype && p->param_dtype != BEVK_DTYPE_F32)
+    return fail(BEVK_ERR_UNSUPPORTED,
+                "group_norm_act: parameter dtype must be the tensors' dtype or f32");
+  if (p->batch < 0 || p->pixels < 0 || p->channels <= 0 || p->groups <= 0)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act: bad sizes");
+  if (p->channels % p->groups)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act: groups=%d must divide channels=%d",
+                p->groups, p->channels);
+  if (p->channels >= (1 << 24))
+    return fail(BEVK_ERR_INDEX_OVERFLOW, "group_norm_act: %d channels (below 2^24)", p->channels);
+  if (p->act != BEVK_ACT_NONE && p->act != BEVK_ACT_RELU && p->act != BEVK_ACT_SILU)
+    return fail(BEVK_ERR_UNSUPPORTED, "group_norm_act: activation %d", p->act);
+  if (!(p->eps >= 0.f) || std::isinf(p->eps))
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act: eps must be finite and >= 0");
+  if (p->pixels >= (int64_t(1) << 31) - (1 << 20))
+    return fail(BEVK_ERR_INDEX_OVERFLOW, "group_norm_act: %lld pixels exceed 31-bit indexing",
+                static_cast<long long>(p->pixels));
+  for (int i = 0; i < 2; ++i)
+    if (p->input_strides[i] < 0 || p->output_strides[i] < 0 ||
+        (backward && p->grad_output_strides[i] < 0))
+      return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act: negative strides");
+  return BEVK_OK;
+}
+
+cudaStream_t cuda_stream(bevk_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
+
+int zero(void *p, size_t bytes, cudaStream_t stream, const char *what) {
+  if (p == nullptr || bytes == 0) return BEVK_OK;
+  return launched(cudaMemsetAsync(p, 0, bytes, stream), what);
+}
+
+}  // namespace
+
+extern "C" {
+
+BEVK_API size_t bevk_group_norm_act_workspace_bytes(const bevk_group_norm_problem *p,
+                                                    int backward) {
+  clear_error();
+  if (check_group_norm(p, backward != 0) != BEVK_OK) return 0;
+  if (p->batch == 0 || p->pixels == 0) return 0;
+  return group_norm_workspace_bytes(p, backward != 0);
+}
+
+BEVK_API int bevk_group_norm_act_forward(const bevk_group_norm_problem *p, const void *input,
+                                         const void *weight, const void *bias, void *output,
+                                         float *mean, float *rstd, void *workspace,
+                                         size_t workspace_bytes, bevk_stream_t stream) {
+  clear_error();
+  const int st = check_group_norm(p, false);
+  if (st != BEVK_OK) return st;
+  if ((mean == nullptr) != (rstd == nullptr))
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act_forward: mean and rstd go together");
+  if (p->batch == 0) return BEVK_OK;
+  if (p->pixels == 0) {
+    const size_t n = sizeof(float) * static_cast<size_t>(p->batch) * p->groups;
+    const int s = zero(mean, n, cuda_stream(stream), "group_norm_act_forward");
+    return s != BEVK_OK ? s : zero(rstd, n, cuda_stream(stream), "group_norm_act_forward");
+  }
+  if (!input || !output || !workspace)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act_forward: null pointer");
+  if (!aligned(workspace, 16))
+    return fail(BEVK_ERR_MISALIGNED, "group_norm_act_forward: workspace must be 16-byte aligned");
+  return launch_group_norm_forward(p, input, weight, bias, output, mean, rstd, workspace,
+                                   workspace_bytes, cuda_stream(stream));
+}
+
+BEVK_API int bevk_group_norm_act_backward(const bevk_group_norm_problem *p,
+                                          const void *grad_output, const void *input,
+                                          const float *mean, const float *rstd,
+                                          const void *weight, const void *bias,
+                                          void *grad_input, void *grad_weight, void *grad_bias,
+                                          void *workspace, size_t workspace_bytes,
+                                          bevk_stream_t stream) {
+  clear_error();
+  const int st = check_group_norm(p, true);
+  if (st != BEVK_OK) return st;
+  if (!grad_input && !grad_weight && !grad_bias) return BEVK_OK;
+  if (p->batch == 0 || p->pixels == 0) {
+    const size_t n = dtype_size(p->param_dtype) * static_cast<size_t>(p->channels);
+    const int s = zero(grad_weight, n, cuda_stream(stream), "group_norm_act_backward");
+    return s != BEVK_OK ? s : zero(grad_bias, n, cuda_stream(stream), "group_norm_act_backward");
+  }
+  if (!grad_output || !input || !mean || !rstd || !workspace)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "group_norm_act_backward: null pointer");
+  if (!aligned(workspace, 16))
+    return fail(BEVK_ERR_MISALIGNED, "group_norm_act_backward: workspace must be 16-byte aligned");
+  return launch_group_norm_backward(p, grad_output, input, mean, rstd, weight, bias, grad_input,
+                                    grad_weight, grad_bias, workspace, workspace_bytes,
+                                    cuda_stream(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,176 @@
+// torch_ext_train.cpp -- module _bevk_train_ext: the training-side operators
+// (group norm with activation on channels-last tensors) over the C ABI.
+#include <optional>
+#include <string>
+#include <tuple>
+
+#include "torch_ext_common.h"
+
+using at::Tensor;
+using namespace bevk_ext;
+
+namespace {
+
+using OptTensor = std::optional<Tensor>;
+
+// Integers go into messages as text: streaming one from an extension crashes
+// where the interpreter has loaded another C++ runtime library than the one
+// that the extension was built with.
+std::string str(int64_t v) { return std::to_string(v); }
+
+// ------------------------------------------------------- group norm + act
+
+// Whether the tensor can be addressed as {image, pixel} strides with channel
+// stride 1: the spatial axes flatten, the channels are consecutive.
+bool channels_last_rows(const Tensor &t) {
+  if (t.size(1) > 1 && t.stride(1) != 1) return false;
+  int64_t inner = -1;  // stride that the next outer spatial axis must have
+  for (int64_t d = t.dim() - 1; d >= 2; --d) {
+    if (t.size(d) == 1) continue;
+    if (inner >= 0 && t.stride(d) != inner) return false;
+    inner = t.stride(d) * t.size(d);
+  }
+  return true;
+}
+
+// A channels-last tensor of t's shape (any number of spatial axes).
+Tensor empty_channels_last(const Tensor &t, at::ScalarType dtype) {
+  std::vector<int64_t> sizes = t.sizes().vec(), strides(sizes.size());
+  int64_t step = 1;
+  strides[1] = 1;
+  step = sizes[1];
+  for (int64_t d = t.dim() - 1; d >= 2; --d) {
+    strides[d] = step;
+    step *= sizes[d];
+  }
+  strides[0] = step;
+  return at::empty_strided(sizes, strides, t.options().dtype(dtype));
+}
+
+Tensor as_channels_last(const Tensor &t) {
+  if (channels_last_rows(t)) return t;
+  Tensor out = empty_channels_last(t, t.scalar_type());
+  out.copy_(t);
+  return out;
+}
+
+void row_strides(const Tensor &t, int64_t strides[2]) {
+  strides[0] = t.size(0) > 1 ? t.stride(0) : 0;
+  strides[1] = 0;
+  for (int64_t d = t.dim() - 1; d >= 2; --d)
+    if (t.size(d) > 1) {
+      strides[1] = t.stride(d);
+      break;
+    }
+  // a single pixel or image is never stepped over
+}
+
+const void *ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
+
+bevk_group_norm_problem gn_problem(const Tensor &input, int64_t num_groups,
+                                   const OptTensor &weight, const OptTensor &bias, double eps,
+                                   int64_t act) {
+  check_cuda(input, "input");
+  TORCH_CHECK(input.dim() >= 2, "bevk: input must be [N, C, *spatial]");
+  TORCH_CHECK(num_groups > 0 && input.size(1) > 0 && input.size(1) % num_groups == 0,
+              "bevk: num_groups=", str(num_groups), " must divide the channels (",
+              str(input.size(1)), ")");
+  TORCH_CHECK(input.size(0) < (int64_t(1) << 31) && input.size(1) < (int64_t(1) << 24),
+              "bevk: input is too large");
+  bevk_group_norm_problem p = {};
+  p.dtype = dtype_of(input);
+  p.param_dtype = p.dtype;
+  bool first = true;
+  for (const OptTensor *t : {&weight, &bias}) {
+    if (!*t) continue;
+    check_same_device(input, **t, "weight / bias");
+    TORCH_CHECK((*t)->dim() == 1 && (*t)->size(0) == input.size(1) && (*t)->is_contiguous(),
+                "bevk: weight and bias must be contiguous [C]");
+    const int dt = dtype_of(**t);
+    TORCH_CHECK(first || dt == p.param_dtype, "bevk: weight and bias must share a dtype");
+    p.param_dtype = dt;
+    first = false;
+  }
+  p.batch = static_cast<int>(input.size(0));
+  p.channels = static_cast<int>(input.size(1));
+  p.groups = static_cast<int>(num_groups);
+  p.act = static_cast<int>(act);
+  p.pixels = 1;
+  for (int64_t d = 2; d < input.dim(); ++d) p.pixels *= input.size(d);
+  p.eps = static_cast<float>(eps);
+  return p;
+}
+
+Tensor scratch(size_t bytes, const Tensor &like) {
+  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+
+std::tuple<Tensor, OptTensor, OptTensor> group_norm_act_forward(
+    const Tensor &input_, int64_t num_groups, const OptTensor &weight, const OptTensor &bias,
+    double eps, int64_t act, bool stats) {
+  bevk_group_norm_problem p = gn_problem(input_, num_groups, weight, bias, eps, act);
+  const c10::cuda::CUDAGuard guard(input_.device());
+  const Tensor input = as_channels_last(input_);
+  Tensor output = empty_channels_last(input, input.scalar_type());
+  row_strides(input, p.input_strides);
+  row_strides(output, p.output_strides);
+  OptTensor mean, rstd;
+  if (stats) {
+    const auto opt = input.options().dtype(at::kFloat);
+    mean = at::empty({input.size(0), num_groups}, opt);
+    rstd = at::empty({input.size(0), num_groups}, opt);
+  }
+  const size_t bytes = bevk_group_norm_act_workspace_bytes(&p, 0);
+  const Tensor ws = scratch(bytes, input);
+  check_status(bevk_group_norm_act_forward(
+                   &p, input.data_ptr(), ptr(weight), ptr(bias), output.data_ptr(),
+                   stats ? mean->data_ptr<float>() : nullptr,
+                   stats ? rstd->data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
+                   current_stream(input)),
+               "group_norm_act_forward");
+  return {output, mean, rstd};
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(
+    const Tensor &grad_output_, const Tensor &input_, const Tensor &mean, const Tensor &rstd,
+    int64_t num_groups, const OptTensor &weight, const OptTensor &bias, int64_t act,
+    bool need_input, bool need_weight, bool need_bias) {
+  bevk_group_norm_problem p = gn_problem(input_, num_groups, weight, bias, 0.0, act);
+  for (const Tensor *t : {&grad_output_, &mean, &rstd})
+    check_same_device(input_, *t, "group norm tensor");
+  TORCH_CHECK(grad_output_.sizes() == input_.sizes() &&
+                  grad_output_.scalar_type() == input_.scalar_type(),
+              "bevk: grad_output must have input's shape and dtype");
+  for (const Tensor *t : {&mean, &rstd})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 2 &&
+                    t->size(0) == input_.size(0) && t->size(1) == num_groups,
+                "bevk: mean and rstd must be contiguous fp32 [N, num_groups]");
+  const c10::cuda::CUDAGuard guard(input_.device());
+  const Tensor input = as_channels_last(input_), grad_output = as_channels_last(grad_output_);
+  row_strides(input, p.input_strides);
+  row_strides(grad_output, p.grad_output_strides);
+  OptTensor gi, gw, gb;
+  if (need_input) {
+    gi = empty_channels_last(input, input.scalar_type());
+    row_strides(*gi, p.output_strides);
+  }
+  const auto popt = weight ? weight->options() : bias ? bias->options() : input.options();
+  if (need_weight) gw = at::empty({input.size(1)}, popt);
+  if (need_bias) gb = at::empty({input.size(1)}, popt);
+  const size_t bytes = bevk_group_norm_act_workspace_bytes(&p, 1);
+  const Tensor ws = scratch(bytes, input);
+  const auto out = [](const OptTensor &t) { return t ? t->data_ptr() : nullptr; };
+  check_status(bevk_group_norm_act_backward(
+                   &p, grad_output.data_ptr(), input.data_ptr(), mean.data_ptr<float>(),
+                   rstd.data_ptr<float>(), ptr(weight), ptr(bias), out(gi), out(gw), out(gb),
+                   ws.data_ptr(), bytes, current_stream(input)),
+               "group_norm_act_backward");
+  return {gi, gw, gb};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("group_norm_act_forward", &group_norm_act_forward);
+  m.def("group_norm_act_backward", &group_norm_act_backward);
+}

@@ -2,7 +2,7 @@
 
     python setup.py build_ext --inplace
 
-Both are plain C++ over libbevk.so (the C ABI in include/bevk.h); they hold
+They are plain C++ over libbevk.so (the C ABI in include/bevk.h); they hold
 no CUDA kernels of their own and are linked with an $ORIGIN rpath so the
 library is found next to them.
 """
@@ -32,6 +32,7 @@ setup(
     ext_modules=[
         ext("_modulated_deform_conv_ext", "torch_ext_dcn.cpp"),
         ext("_ms_deform_attn_ext", "torch_ext_msda.cpp"),
+        ext("_bevk_train_ext", "torch_ext_train.cpp"),
     ],
     cmdclass={"build_ext": BuildExtension},
 )

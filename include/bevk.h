@@ -471,6 +471,68 @@ BEVK_API int bevk_ms_deform_attn_backward(
     void *grad_sampling_loc, void *grad_attention_weights, void *workspace,
     size_t workspace_bytes, int dtype, bevk_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Training-side operators (no counterpart in the reference)                 */
+/* ------------------------------------------------------------------------ */
+
+/* Activation fused behind the group norm. */
+enum bevk_activation {
+  BEVK_ACT_NONE = 0,
+  BEVK_ACT_RELU = 1,
+  BEVK_ACT_SILU = 2 /* z * sigmoid(z) */
+};
+
+/*
+ * Group norm followed by an activation on channels-last tensors:
+ *   z = weight[c] * (x - mean[n, g]) * rstd[n, g] + bias[c],   y = act(z),
+ * mean and rstd = 1 / sqrt(var + eps) (biased variance) over the pixels and
+ * the channels / groups channels of group g of image n.
+ *
+ * Every 4-D tensor has channel stride 1 and is addressed by two element
+ * strides: {image, pixel}, pixel < pixels running over the flattened spatial
+ * positions.  fp32, fp16 or bf16; weight and bias share param_dtype, which is
+ * the tensors' dtype or fp32.  Statistics and sums are fp32; results are
+ * rounded once.  Runs of equal inputs give equal bits (no atomics).
+ */
+typedef struct bevk_group_norm_problem {
+  int dtype;                     /* enum bevk_dtype of input, output, gradients */
+  int param_dtype;               /* of weight, bias and their gradients         */
+  int batch, channels, groups;
+  int act;                       /* enum bevk_activation                        */
+  int64_t pixels;                /* spatial positions of one image              */
+  float eps;
+  int64_t input_strides[2];
+  int64_t output_strides[2];     /* forward: output; backward: grad_input       */
+  int64_t grad_output_strides[2];/* backward                                    */
+} bevk_group_norm_problem;
+
+/* Scratch bytes of the forward (backward = 0) or backward (1) call on this
+ * problem; 16-byte aligned, contents need no initialisation.  0 on a bad
+ * problem. */
+BEVK_API size_t bevk_group_norm_act_workspace_bytes(const bevk_group_norm_problem *p,
+                                                    int backward);
+/*
+ * Writes output, and mean and rstd ([batch, groups] fp32) unless both are
+ * NULL.  weight and bias may be NULL (1 and 0).  With no pixels nothing but
+ * zero statistics is written.
+ */
+BEVK_API int bevk_group_norm_act_forward(const bevk_group_norm_problem *p, const void *input,
+                                         const void *weight, const void *bias, void *output,
+                                         float *mean, float *rstd, void *workspace,
+                                         size_t workspace_bytes, bevk_stream_t stream);
+/*
+ * Gradients of the call above from the statistics it wrote.  grad_input,
+ * grad_weight and grad_bias may each be NULL (not computed); weight and bias
+ * are the forward's (bias is read for the activation's argument only).
+ */
+BEVK_API int bevk_group_norm_act_backward(const bevk_group_norm_problem *p,
+                                          const void *grad_output, const void *input,
+                                          const float *mean, const float *rstd,
+                                          const void *weight, const void *bias,
+                                          void *grad_input, void *grad_weight, void *grad_bias,
+                                          void *workspace, size_t workspace_bytes,
+                                          bevk_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,80 @@
+"""Training-side operators on a host without a GPU: argument checks of the C ABI
+(all made before a device is touched), no CPU fallback, module construction."""
+import ctypes
+
+import pytest
+import torch
+
+import group_norm_act as gna
+from bevk import cabi
+
+
+def _gn(**kw):
+    p = cabi.GroupNormProblem()
+    p.dtype, p.param_dtype = cabi.DTYPE_F16, cabi.DTYPE_F32
+    p.batch, p.channels, p.groups, p.pixels = 2, 64, 8, 100
+    p.act, p.eps = cabi.ACT_SILU, 1e-5
+    for name in ("input_strides", "output_strides", "grad_output_strides"):
+        getattr(p, name)[0], getattr(p, name)[1] = 6400, 64
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(groups=7), cabi.ERR_INVALID_ARGUMENT, "divide"),
+    (dict(groups=0), cabi.ERR_INVALID_ARGUMENT, "sizes"),
+    (dict(channels=0), cabi.ERR_INVALID_ARGUMENT, "sizes"),
+    (dict(batch=-1), cabi.ERR_INVALID_ARGUMENT, "sizes"),
+    (dict(dtype=cabi.DTYPE_F64), cabi.ERR_UNSUPPORTED, "dtype"),
+    (dict(param_dtype=cabi.DTYPE_BF16), cabi.ERR_UNSUPPORTED, "parameter dtype"),
+    (dict(act=7), cabi.ERR_UNSUPPORTED, "activation"),
+    (dict(eps=float("nan")), cabi.ERR_INVALID_ARGUMENT, "eps"),
+    (dict(eps=-1.0), cabi.ERR_INVALID_ARGUMENT, "eps"),
+    (dict(pixels=1 << 31), cabi.ERR_INDEX_OVERFLOW, "pixels"),
+])
+def test_group_norm_problem_validation(kw, status, word):
+    L, p = cabi.lib(), _gn(**kw)
+    assert L.bevk_group_norm_act_workspace_bytes(ctypes.byref(p), 0) == 0
+    st = L.bevk_group_norm_act_forward(ctypes.byref(p), 16, None, None, 16, None, None, 16, 1 << 20,
+                                       None)
+    assert st == status and word in cabi.last_error()
+    st = L.bevk_group_norm_act_backward(ctypes.byref(p), 16, 16, 16, 16, None, None, 16, None, None,
+                                        16, 1 << 20, None)
+    assert st == status
+
+
+def test_group_norm_pointer_checks():
+    L, p = cabi.lib(), _gn()
+    assert L.bevk_group_norm_act_workspace_bytes(ctypes.byref(p), 0) > 0
+    assert L.bevk_group_norm_act_workspace_bytes(ctypes.byref(p), 1) > 0
+    ref = ctypes.byref(p)
+    assert L.bevk_group_norm_act_forward(ref, None, None, None, 16, None, None, 16, 1 << 20,
+                                         None) == cabi.ERR_INVALID_ARGUMENT
+    assert L.bevk_group_norm_act_forward(ref, 16, None, None, 16, 16, None, 16, 1 << 20,
+                                         None) == cabi.ERR_INVALID_ARGUMENT
+    assert L.bevk_group_norm_act_forward(ref, 16, None, None, 16, None, None, 8, 1 << 20,
+                                         None) == cabi.ERR_MISALIGNED
+    assert L.bevk_group_norm_act_forward(None, 16, None, None, 16, None, None, 16, 1 << 20,
+                                         None) == cabi.ERR_INVALID_ARGUMENT
+    # nothing to do
+    empty = _gn(batch=0)
+    assert L.bevk_group_norm_act_forward(ctypes.byref(empty), None, None, None, None, None, None,
+                                         None, 0, None) == cabi.OK
+    assert L.bevk_group_norm_act_backward(ref, 16, 16, 16, 16, None, None, None, None, None, None,
+                                          0, None) == cabi.OK
+
+
+def test_group_norm_module_and_no_cpu_fallback():
+    m = gna.GroupNormAct(8, 32, act="relu")
+    assert set(m.state_dict()) == {"weight", "bias"} and "relu" in repr(m)
+    assert not gna.GroupNormAct(8, 32, affine=False).state_dict()
+    with pytest.raises(ValueError):
+        gna.GroupNormAct(5, 32)
+    with pytest.raises(ValueError, match="act"):
+        gna.GroupNormAct(8, 32, act="tanh")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        m(torch.randn(1, 32, 2, 2))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        gna.group_norm_act_backward(*[torch.randn(1, 32, 2, 2)] * 2, torch.ones(1, 8),
+                                    torch.ones(1, 8), 8)
