@@ -54,6 +54,8 @@ EXPORTED_SYMBOLS = (
     "bevk_group_norm_act_workspace_bytes",
     "bevk_group_norm_act_forward",
     "bevk_group_norm_act_backward",
+    "bevk_grad_clip_workspace_bytes",
+    "bevk_grad_clip",
 )
 
 
@@ -131,6 +133,16 @@ class GroupNormProblem(ctypes.Structure):
     ]
 
 
+NORM_L2, NORM_INF = 0, 1
+
+
+class GradTensor(ctypes.Structure):
+    """Mirror of ``bevk_grad_tensor``."""
+
+    _fields_ = [("grad", ctypes.c_void_p), ("out", ctypes.c_void_p), ("numel", ctypes.c_int64),
+                ("grad_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int)]
+
+
 class BevkError(RuntimeError):
     def __init__(self, status: int, what: str, detail: str):
         super().__init__(f"{what}: {status_string(status)} ({status}): {detail}")
@@ -204,6 +216,11 @@ def lib():
     L.bevk_group_norm_act_forward.argtypes = [gp] + [vp] * 7 + [sz, vp]
     L.bevk_group_norm_act_backward.restype = i
     L.bevk_group_norm_act_backward.argtypes = [gp] + [vp] * 10 + [sz, vp]
+    f = ctypes.c_float
+    L.bevk_grad_clip_workspace_bytes.restype = sz
+    L.bevk_grad_clip_workspace_bytes.argtypes = [i]
+    L.bevk_grad_clip.restype = i
+    L.bevk_grad_clip.argtypes = [ctypes.POINTER(GradTensor), i, i, f, f, i, vp, vp, sz, vp]
     _lib = L
     return L
 

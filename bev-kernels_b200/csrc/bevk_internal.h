@@ -154,6 +154,11 @@ int launch_group_norm_backward(const bevk_group_norm_problem *q, const void *dy,
                                void *dx, void *dw, void *db, void *ws, size_t ws_bytes,
                                cudaStream_t stream);
 
+// Global gradient norm and clipping (grad_clip.cu).
+size_t grad_clip_workspace_bytes(int tensors);
+int launch_grad_clip(const bevk_grad_tensor *tensors, int n, int norm_kind, float max_norm,
+                     float eps, int scale, float *norm_out, void *ws, cudaStream_t stream);
+
 // Device watchdog word (one per device, defined in dcn_tc.cu).
 int read_and_clear_watchdog(int device, unsigned int *code);
 // Limit of the fused DCN kernel's pipeline barrier waits on `device` (0: the

@@ -112,4 +112,45 @@ BEVK_API int bevk_group_norm_act_backward(const bevk_group_norm_problem *p,
                                     cuda_stream(stream));
 }
 
+BEVK_API size_t bevk_grad_clip_workspace_bytes(int num_tensors) {
+  clear_error();
+  return num_tensors < 0 ? 0 : grad_clip_workspace_bytes(num_tensors);
+}
+
+BEVK_API int bevk_grad_clip(const bevk_grad_tensor *tensors, int num_tensors, int norm_kind,
+                            float max_norm, float eps, int scale, float *norm_out,
+                            void *workspace, size_t workspace_bytes, bevk_stream_t stream) {
+  clear_error();
+  if (num_tensors < 0 || (num_tensors > 0 && !tensors) || !norm_out)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "grad_clip: null pointer or negative count");
+  if (norm_kind != BEVK_NORM_L2 && norm_kind != BEVK_NORM_INF)
+    return fail(BEVK_ERR_UNSUPPORTED, "grad_clip: norm kind %d", norm_kind);
+  if (scale && (!(max_norm >= 0.f) || !(eps >= 0.f)))
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "grad_clip: max_norm and eps must be >= 0");
+  int64_t total = 0;
+  for (int i = 0; i < num_tensors; ++i) {
+    const bevk_grad_tensor &t = tensors[i];
+    if (t.numel < 0) return fail(BEVK_ERR_INVALID_ARGUMENT, "grad_clip: tensor %d: numel", i);
+    if (!known_dtype(t.grad_dtype) || (scale && !known_dtype(t.out_dtype)))
+      return fail(BEVK_ERR_UNSUPPORTED, "grad_clip: tensor %d: dtype (f32, f16, bf16)", i);
+    if (t.numel == 0) continue;
+    if (!t.grad || (scale && !t.out))
+      return fail(BEVK_ERR_INVALID_ARGUMENT, "grad_clip: tensor %d: null pointer", i);
+    if (!aligned(t.grad, dtype_size(t.grad_dtype)) ||
+        (scale && !aligned(t.out, dtype_size(t.out_dtype))))
+      return fail(BEVK_ERR_MISALIGNED, "grad_clip: tensor %d: not aligned to its type", i);
+    if (scale && t.grad == t.out && t.grad_dtype != t.out_dtype)
+      return fail(BEVK_ERR_INVALID_ARGUMENT, "grad_clip: tensor %d: in place with two types", i);
+    total += t.numel;
+  }
+  if (total == 0) return zero(norm_out, sizeof(float), cuda_stream(stream), "grad_clip");
+  if (!workspace || workspace_bytes < grad_clip_workspace_bytes(num_tensors))
+    return fail(BEVK_ERR_WORKSPACE, "grad_clip: workspace of %zu bytes, needs %zu",
+                workspace_bytes, grad_clip_workspace_bytes(num_tensors));
+  if (!aligned(workspace, 16))
+    return fail(BEVK_ERR_MISALIGNED, "grad_clip: workspace must be 16-byte aligned");
+  return launch_grad_clip(tensors, num_tensors, norm_kind, max_norm, eps, scale, norm_out,
+                          workspace, cuda_stream(stream));
+}
+
 }  // extern "C"

@@ -1,8 +1,10 @@
 // torch_ext_train.cpp -- module _bevk_train_ext: the training-side operators
-// (group norm with activation on channels-last tensors) over the C ABI.
+// (group norm with activation on channels-last tensors, the global gradient
+// norm and clipping) over the C ABI.
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "torch_ext_common.h"
 
@@ -168,9 +170,90 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(
   return {gi, gw, gb};
 }
 
+// ------------------------------------------------ gradient norm and clipping
+
+bool dense(const Tensor &t) { return t.is_non_overlapping_and_dense(); }
+
+// A dense tensor of like's strides (contiguous where like has holes).
+Tensor empty_dense(const Tensor &like, at::ScalarType dtype) {
+  return dense(like) ? at::empty_strided(like.sizes(), like.strides(), like.options().dtype(dtype))
+                     : at::empty(like.sizes(), like.options().dtype(dtype));
+}
+
+// The norm of all tensors; where max_norm is given, also scales them, into
+// `out` or in place.  Tensors with holes, and outputs of another layout than
+// their gradient's, go through a dense copy.
+Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_norm, double eps,
+                 bool inf_norm, const std::optional<std::vector<Tensor>> &out) {
+  TORCH_CHECK(!grads.empty(), "bevk: no gradients");
+  TORCH_CHECK(!out || out->size() == grads.size(), "bevk: one output for each gradient");
+  const Tensor &first = grads[0];
+  std::vector<bevk_grad_tensor> items(grads.size());
+  std::vector<Tensor> keep;                          // copies the call reads or writes
+  std::vector<std::pair<Tensor, Tensor>> copy_back;  // (to, from)
+  const c10::cuda::OptionalCUDAGuard guard(first.is_cuda() ? std::optional<c10::Device>(first.device())
+                                                           : std::nullopt);
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor &g = grads[i];
+    check_cuda(g, "gradient");
+    check_same_device(first, g, "gradient");
+    TORCH_CHECK(g.layout() == at::kStrided, "bevk: gradients must be strided tensors");
+    bevk_grad_tensor &it = items[i];
+    it.grad_dtype = dtype_of(g);
+    it.numel = g.numel();
+    Tensor src = g;
+    if (!max_norm) {
+      if (!dense(src)) keep.push_back(src = src.contiguous());
+      it.grad = it.out = src.data_ptr();
+      it.out_dtype = it.grad_dtype;
+      continue;
+    }
+    const Tensor &o = out ? (*out)[i] : g;
+    if (out) {
+      check_same_device(first, o, "output");
+      TORCH_CHECK(o.sizes() == g.sizes(), "bevk: an output must have its gradient's shape");
+    }
+    for (int64_t d = 0; d < o.dim(); ++d)
+      TORCH_CHECK(o.numel() == 0 || o.size(d) == 1 || o.stride(d) != 0,
+                  "bevk: an expanded tensor cannot be written");
+    const bool in_place = o.data_ptr() == g.data_ptr() && o.scalar_type() == g.scalar_type() &&
+                          o.strides() == g.strides();
+    Tensor dst = o;
+    if (!dense(dst)) {
+      keep.push_back(dst = empty_dense(o, o.scalar_type()));
+      copy_back.emplace_back(o, dst);
+    }
+    if (in_place) {
+      if (!dst.is_same(o)) {
+        dst.copy_(src);
+        src = dst;
+      }
+    } else if (!dense(src) || src.strides() != dst.strides()) {
+      Tensor c = empty_dense(dst, src.scalar_type());
+      c.copy_(src);
+      keep.push_back(src = c);
+    }
+    it.grad = src.data_ptr();
+    it.out = dst.data_ptr();
+    it.out_dtype = dtype_of(dst);
+  }
+  Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
+  const size_t bytes = bevk_grad_clip_workspace_bytes(static_cast<int>(items.size()));
+  const Tensor ws = scratch(bytes, first);
+  check_status(bevk_grad_clip(items.data(), static_cast<int>(items.size()),
+                              inf_norm ? BEVK_NORM_INF : BEVK_NORM_L2,
+                              static_cast<float>(max_norm.value_or(0.0)), static_cast<float>(eps),
+                              max_norm.has_value(), norm.data_ptr<float>(), ws.data_ptr(), bytes,
+                              current_stream(first)),
+               "grad_clip");
+  for (auto &c : copy_back) c.first.copy_(c.second);
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm_act_forward", &group_norm_act_forward);
   m.def("group_norm_act_backward", &group_norm_act_backward);
+  m.def("grad_clip", &grad_clip);
 }

@@ -533,6 +533,33 @@ BEVK_API int bevk_group_norm_act_backward(const bevk_group_norm_problem *p,
                                           void *workspace, size_t workspace_bytes,
                                           bevk_stream_t stream);
 
+/* One tensor of bevk_grad_clip: numel contiguous elements. */
+typedef struct bevk_grad_tensor {
+  const void *grad;
+  void *out;        /* == grad: scaled in place; else a buffer of numel elements */
+  int64_t numel;
+  int grad_dtype, out_dtype; /* fp32, fp16, bf16 */
+} bevk_grad_tensor;
+
+enum bevk_norm_kind { BEVK_NORM_L2 = 0, BEVK_NORM_INF = 1 };
+
+/* Scratch bytes of bevk_grad_clip; 16-byte aligned, needs no initialisation. */
+BEVK_API size_t bevk_grad_clip_workspace_bytes(int num_tensors);
+/*
+ * The norm over all elements of all tensors, and clipping by it:
+ *   norm = sqrt(sum g^2) or max |g|,  c = min(1, max_norm / (norm + eps)),
+ *   out = c * g (rounded once),  norm_out[0] = norm (fp32, device memory).
+ * scale = 0 only takes the norm (out is ignored).  A NaN in any gradient makes
+ * the norm NaN and with it every output; an infinite norm gives c = 0.  In
+ * place, c = 1 writes nothing.  Squares are fp32 and their sums fp64: a
+ * gradient above 1.8e19 makes the norm infinite.  Outputs must not overlap one another, nor a
+ * gradient other than their own.  tensors is host memory, read before the
+ * call returns.  Equal inputs give equal bits (no floating-point atomics).
+ */
+BEVK_API int bevk_grad_clip(const bevk_grad_tensor *tensors, int num_tensors, int norm_kind,
+                            float max_norm, float eps, int scale, float *norm_out,
+                            void *workspace, size_t workspace_bytes, bevk_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

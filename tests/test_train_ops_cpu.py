@@ -5,6 +5,7 @@ import ctypes
 import pytest
 import torch
 
+import grad_clip
 import group_norm_act as gna
 from bevk import cabi
 
@@ -78,3 +79,42 @@ def test_group_norm_module_and_no_cpu_fallback():
     with pytest.raises(RuntimeError, match="CUDA"):
         gna.group_norm_act_backward(*[torch.randn(1, 32, 2, 2)] * 2, torch.ones(1, 8),
                                     torch.ones(1, 8), 8)
+
+
+def test_grad_clip_checks():
+    L = cabi.lib()
+    assert L.bevk_grad_clip_workspace_bytes(0) > 0
+    assert L.bevk_grad_clip_workspace_bytes(2300) > L.bevk_grad_clip_workspace_bytes(1000)
+    t = (cabi.GradTensor * 2)()
+    for k in range(2):
+        t[k].grad, t[k].out, t[k].numel = 4096, 4096, 8
+
+    def call(n=2, kind=0, limit=1.0, scale=1, norm=16, ws=16, nbytes=1 << 20):
+        return L.bevk_grad_clip(t, n, kind, limit, 1e-6, scale, norm, ws, nbytes, None)
+
+    assert call() == cabi.ERR_INVALID_ARGUMENT and "overlaps" in cabi.last_error()
+    t[1].grad = t[1].out = 4096 + 32
+    assert call(kind=2) == cabi.ERR_UNSUPPORTED
+    assert call(limit=-1.0) == cabi.ERR_INVALID_ARGUMENT
+    assert call(limit=float("nan")) == cabi.ERR_INVALID_ARGUMENT
+    assert call(norm=None) == cabi.ERR_INVALID_ARGUMENT
+    assert call(n=-1) == cabi.ERR_INVALID_ARGUMENT
+    assert call(nbytes=8) == cabi.ERR_WORKSPACE
+    assert call(ws=None) == cabi.ERR_WORKSPACE
+    assert call(ws=24) == cabi.ERR_MISALIGNED
+    t[1].out = 4096 + 24                     # overlaps the first tensor, which is written
+    assert call() == cabi.ERR_INVALID_ARGUMENT
+    t[1].out = t[1].grad
+    t[1].grad_dtype, t[1].out_dtype = cabi.DTYPE_F16, cabi.DTYPE_F32
+    assert call() == cabi.ERR_INVALID_ARGUMENT and "two types" in cabi.last_error()
+    t[1].grad_dtype = cabi.DTYPE_F64
+    assert call() == cabi.ERR_UNSUPPORTED
+    t[1].numel = -1
+    assert call() == cabi.ERR_INVALID_ARGUMENT
+    with pytest.raises(RuntimeError, match="CUDA"):
+        grad_clip.grad_norm([torch.ones(3)])
+    with pytest.raises(ValueError, match="norm_type"):
+        grad_clip.clip_grads([torch.ones(3)], 1.0, norm_type=3)
+    with pytest.raises(TypeError):
+        grad_clip.clip_grad_norm_(3.0, 1.0)
+    assert float(grad_clip.clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0)) == 0.0
