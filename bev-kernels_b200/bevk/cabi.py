@@ -54,6 +54,9 @@ EXPORTED_SYMBOLS = (
     "bevk_group_norm_act_workspace_bytes",
     "bevk_group_norm_act_forward",
     "bevk_group_norm_act_backward",
+    "bevk_embedding_forward",
+    "bevk_embedding_backward_workspace_bytes",
+    "bevk_embedding_backward",
     "bevk_grad_clip_workspace_bytes",
     "bevk_grad_clip",
 )
@@ -130,6 +133,20 @@ class GroupNormProblem(ctypes.Structure):
         ("input_strides", ctypes.c_int64 * 2),
         ("output_strides", ctypes.c_int64 * 2),
         ("grad_output_strides", ctypes.c_int64 * 2),
+    ]
+
+
+class EmbeddingBackwardArgs(ctypes.Structure):
+    """Mirror of ``bevk_embedding_backward_args``."""
+
+    _fields_ = [
+        ("num_ids", ctypes.c_int64), ("num_rows", ctypes.c_int64),
+        ("dim", ctypes.c_int), ("ids_are_64bit", ctypes.c_int),
+        ("grad_output_ld", ctypes.c_int64), ("grad_table_ld", ctypes.c_int64),
+        ("padding_idx", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("grad_output_dtype", ctypes.c_int), ("grad_table_dtype", ctypes.c_int),
+        ("accumulate", ctypes.c_int),
     ]
 
 
@@ -216,7 +233,14 @@ def lib():
     L.bevk_group_norm_act_forward.argtypes = [gp] + [vp] * 7 + [sz, vp]
     L.bevk_group_norm_act_backward.restype = i
     L.bevk_group_norm_act_backward.argtypes = [gp] + [vp] * 10 + [sz, vp]
-    f = ctypes.c_float
+    f, i64 = ctypes.c_float, ctypes.c_int64
+    ep = ctypes.POINTER(EmbeddingBackwardArgs)
+    L.bevk_embedding_forward.restype = i
+    L.bevk_embedding_forward.argtypes = [vp, i64, vp, i, i64, i64, i, f, vp, i, vp]
+    L.bevk_embedding_backward_workspace_bytes.restype = sz
+    L.bevk_embedding_backward_workspace_bytes.argtypes = [ep]
+    L.bevk_embedding_backward.restype = i
+    L.bevk_embedding_backward.argtypes = [ep, vp, vp, vp, vp, sz, vp]
     L.bevk_grad_clip_workspace_bytes.restype = sz
     L.bevk_grad_clip_workspace_bytes.argtypes = [i]
     L.bevk_grad_clip.restype = i

@@ -154,6 +154,14 @@ int launch_group_norm_backward(const bevk_group_norm_problem *q, const void *dy,
                                void *dx, void *dw, void *db, void *ws, size_t ws_bytes,
                                cudaStream_t stream);
 
+// Embedding lookup with scaling and its gradient (embedding.cu).
+int launch_embedding_forward(const void *table, int64_t ld, const void *ids, bool wide_ids,
+                             int64_t n, int64_t rows, int dim, float scale, void *out, int dtype,
+                             cudaStream_t stream);
+size_t embedding_backward_workspace_bytes(const bevk_embedding_backward_args *a);
+int launch_embedding_backward(const bevk_embedding_backward_args *a, const void *dy,
+                              const void *ids, void *grad_table, void *ws, cudaStream_t stream);
+
 // Global gradient norm and clipping (grad_clip.cu).
 size_t grad_clip_workspace_bytes(int tensors);
 int launch_grad_clip(const bevk_grad_tensor *tensors, int n, int norm_kind, float max_norm,

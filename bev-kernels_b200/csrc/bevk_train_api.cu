@@ -45,6 +45,25 @@ int check_group_norm(const bevk_group_norm_problem *p, bool backward) {
   return BEVK_OK;
 }
 
+// Checks the arguments of the embedding gradient (not its pointers).
+int check_embedding_backward(const bevk_embedding_backward_args *a) {
+  if (!a) return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_backward: null arguments");
+  if (!known_dtype(a->grad_output_dtype) ||
+      (a->grad_table_dtype != a->grad_output_dtype && a->grad_table_dtype != BEVK_DTYPE_F32))
+    return fail(BEVK_ERR_UNSUPPORTED,
+                "embedding_backward: dtypes %d -> %d (f32, f16, bf16, into the same or f32)",
+                a->grad_output_dtype, a->grad_table_dtype);
+  if (a->num_ids < 0 || a->num_rows < 0 || a->dim <= 0)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_backward: bad sizes");
+  if (a->grad_output_ld < 0 || a->grad_table_ld < a->dim)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_backward: bad row strides");
+  if (a->num_ids >= (int64_t(1) << 31) - (1 << 16) || a->num_rows >= (int64_t(1) << 31) - 1 ||
+      a->dim >= (1 << 24))
+    return fail(BEVK_ERR_INDEX_OVERFLOW,
+                "embedding_backward: ids and rows are indexed in 31 bits, columns in 24");
+  return BEVK_OK;
+}
+
 cudaStream_t cuda_stream(bevk_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 int zero(void *p, size_t bytes, cudaStream_t stream, const char *what) {
@@ -110,6 +129,58 @@ BEVK_API int bevk_group_norm_act_backward(const bevk_group_norm_problem *p,
   return launch_group_norm_backward(p, grad_output, input, mean, rstd, weight, bias, grad_input,
                                     grad_weight, grad_bias, workspace, workspace_bytes,
                                     cuda_stream(stream));
+}
+
+BEVK_API int bevk_embedding_forward(const void *table, int64_t table_ld, const void *ids,
+                                    int ids_are_64bit, int64_t num_ids, int64_t num_rows,
+                                    int dim, float scale, void *output, int dtype,
+                                    bevk_stream_t stream) {
+  clear_error();
+  if (!known_dtype(dtype))
+    return fail(BEVK_ERR_UNSUPPORTED, "embedding_forward: dtype %d (f32, f16, bf16)", dtype);
+  if (num_ids < 0 || num_rows < 0 || dim <= 0 || table_ld < 0)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_forward: bad sizes");
+  if (dim >= (1 << 24))
+    return fail(BEVK_ERR_INDEX_OVERFLOW, "embedding_forward: %d columns (below 2^24)", dim);
+  if (num_ids == 0) return BEVK_OK;
+  if (!ids || !output || (!table && num_rows > 0))
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_forward: null pointer");
+  return launch_embedding_forward(table, table_ld, ids, ids_are_64bit != 0, num_ids, num_rows, dim,
+                                  scale, output, dtype, cuda_stream(stream));
+}
+
+BEVK_API size_t bevk_embedding_backward_workspace_bytes(const bevk_embedding_backward_args *a) {
+  clear_error();
+  if (check_embedding_backward(a) != BEVK_OK || a->num_ids == 0 || a->num_rows == 0) return 0;
+  return embedding_backward_workspace_bytes(a);
+}
+
+BEVK_API int bevk_embedding_backward(const bevk_embedding_backward_args *a,
+                                     const void *grad_output, const void *ids, void *grad_table,
+                                     void *workspace, size_t workspace_bytes,
+                                     bevk_stream_t stream) {
+  clear_error();
+  const int st = check_embedding_backward(a);
+  if (st != BEVK_OK) return st;
+  if (a->num_rows == 0) return BEVK_OK;
+  if (!grad_table) return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_backward: null pointer");
+  if (a->num_ids == 0) {
+    if (a->accumulate) return BEVK_OK;
+    const size_t size = dtype_size(a->grad_table_dtype);
+    return launched(cudaMemset2DAsync(grad_table, a->grad_table_ld * size, 0, a->dim * size,
+                                      a->num_rows, cuda_stream(stream)),
+                    "embedding_backward");
+  }
+  if (!grad_output || !ids)
+    return fail(BEVK_ERR_INVALID_ARGUMENT, "embedding_backward: null pointer");
+  const size_t need = embedding_backward_workspace_bytes(a);
+  if (!workspace || workspace_bytes < need)
+    return fail(BEVK_ERR_WORKSPACE, "embedding_backward: workspace of %zu bytes, needs %zu",
+                workspace_bytes, need);
+  if (!aligned(workspace, 256))
+    return fail(BEVK_ERR_MISALIGNED, "embedding_backward: workspace must be 256-byte aligned");
+  return launch_embedding_backward(a, grad_output, ids, grad_table, workspace,
+                                   cuda_stream(stream));
 }
 
 BEVK_API size_t bevk_grad_clip_workspace_bytes(int num_tensors) {

@@ -1,6 +1,6 @@
 // torch_ext_train.cpp -- module _bevk_train_ext: the training-side operators
-// (group norm with activation on channels-last tensors, the global gradient
-// norm and clipping) over the C ABI.
+// (group norm with activation on channels-last tensors, embedding lookup with
+// scaling, the global gradient norm and clipping) over the C ABI.
 #include <optional>
 #include <string>
 #include <tuple>
@@ -170,6 +170,89 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(
   return {gi, gw, gb};
 }
 
+// ------------------------------------------------------------- embedding
+
+bool wide_ids(const Tensor &ids) {
+  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt,
+              "bevk: ids must be int64 or int32");
+  return ids.scalar_type() == at::kLong;
+}
+
+// t's rows one after the other, or t where they can be addressed as they are.
+Tensor as_rows(const Tensor &t) {
+  return t.dim() == 2 && (t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) >= t.size(1)
+             ? t
+             : t.contiguous();
+}
+int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+Tensor embedding_forward(const Tensor &table, const Tensor &ids_, double scale) {
+  check_cuda(table, "weight");
+  check_same_device(table, ids_, "ids");
+  TORCH_CHECK(table.dim() == 2 && table.size(1) > 0, "bevk: weight must be [rows, dim]");
+  TORCH_CHECK(table.size(1) < (int64_t(1) << 24), "bevk: weight has too many columns");
+  const bool wide = wide_ids(ids_);
+  const int dt = dtype_of(table);
+  const c10::cuda::CUDAGuard guard(table.device());
+  const Tensor rows = as_rows(table), ids = ids_.contiguous();
+  std::vector<int64_t> sizes = ids.sizes().vec();
+  sizes.push_back(table.size(1));
+  Tensor out = at::empty(sizes, table.options());
+  check_status(bevk_embedding_forward(rows.data_ptr(), row_stride(rows), ids.data_ptr(), wide,
+                                      ids.numel(), rows.size(0), static_cast<int>(rows.size(1)),
+                                      static_cast<float>(scale), out.data_ptr(), dt,
+                                      current_stream(table)),
+               "embedding_forward");
+  return out;
+}
+
+// Where `into` is given the gradient is added to it (and it is returned).
+Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t num_rows,
+                          double scale, int64_t padding_idx, const OptTensor &into) {
+  check_cuda(grad_output, "grad_output");
+  check_same_device(grad_output, ids_, "ids");
+  const bool wide = wide_ids(ids_);
+  TORCH_CHECK(grad_output.dim() == ids_.dim() + 1 &&
+                  grad_output.sizes().slice(0, ids_.dim()) == ids_.sizes(),
+              "bevk: grad_output must be [*ids.shape, dim]");
+  const int64_t dim = grad_output.size(-1);
+  TORCH_CHECK(dim > 0 && dim < (int64_t(1) << 24) && num_rows >= 0,
+              "bevk: bad number of rows or columns");
+  bevk_embedding_backward_args a = {};
+  a.grad_output_dtype = dtype_of(grad_output);
+  const c10::cuda::CUDAGuard guard(grad_output.device());
+  const Tensor ids = ids_.contiguous();
+  const Tensor dy = as_rows(grad_output.dim() == 2 ? grad_output : grad_output.reshape({-1, dim}));
+  Tensor out;
+  if (into) {
+    check_same_device(grad_output, *into, "grad_weight");
+    TORCH_CHECK(into->dim() == 2 && into->size(0) == num_rows && into->size(1) == dim,
+                "bevk: grad_weight must be [num_embeddings, dim]");
+    TORCH_CHECK((dim == 1 || into->stride(1) == 1) &&
+                    (num_rows <= 1 || into->stride(0) >= dim),
+                "bevk: grad_weight's rows must be contiguous and apart");
+    out = *into;
+  } else {
+    out = at::empty({num_rows, dim}, grad_output.options());
+  }
+  a.grad_table_dtype = dtype_of(out);
+  a.num_ids = ids.numel();
+  a.num_rows = num_rows;
+  a.dim = static_cast<int>(dim);
+  a.ids_are_64bit = wide;
+  a.grad_output_ld = dy.size(0) > 0 ? row_stride(dy) : dim;
+  a.grad_table_ld = num_rows > 0 ? row_stride(out) : dim;
+  a.padding_idx = padding_idx;
+  a.scale = static_cast<float>(scale);
+  a.accumulate = into.has_value();
+  const size_t bytes = bevk_embedding_backward_workspace_bytes(&a);
+  const Tensor ws = scratch(bytes, grad_output);
+  check_status(bevk_embedding_backward(&a, dy.data_ptr(), ids.data_ptr(), out.data_ptr(),
+                                       ws.data_ptr(), bytes, current_stream(grad_output)),
+               "embedding_backward");
+  return out;
+}
+
 // ------------------------------------------------ gradient norm and clipping
 
 bool dense(const Tensor &t) { return t.is_non_overlapping_and_dense(); }
@@ -255,5 +338,7 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm_act_forward", &group_norm_act_forward);
   m.def("group_norm_act_backward", &group_norm_act_backward);
+  m.def("embedding_forward", &embedding_forward);
+  m.def("embedding_backward", &embedding_backward);
   m.def("grad_clip", &grad_clip);
 }

@@ -533,6 +533,46 @@ BEVK_API int bevk_group_norm_act_backward(const bevk_group_norm_problem *p,
                                           void *workspace, size_t workspace_bytes,
                                           bevk_stream_t stream);
 
+/*
+ * Embedding lookup with scaling: output[i, :] = scale * table[ids[i], :],
+ * computed in fp32 and rounded once.  table has num_rows rows of dim elements
+ * at row stride table_ld; output is [num_ids, dim] contiguous.  ids are int64
+ * (ids_are_64bit = 1) or int32.  An id outside [0, num_rows) reads as a row of
+ * zeros.  table and output share dtype (fp32, fp16, bf16).
+ */
+BEVK_API int bevk_embedding_forward(const void *table, int64_t table_ld, const void *ids,
+                                    int ids_are_64bit, int64_t num_ids, int64_t num_rows,
+                                    int dim, float scale, void *output, int dtype,
+                                    bevk_stream_t stream);
+
+typedef struct bevk_embedding_backward_args {
+  int64_t num_ids, num_rows;
+  int dim;
+  int ids_are_64bit;
+  int64_t grad_output_ld;  /* row stride of grad_output                        */
+  int64_t grad_table_ld;   /* row stride of grad_table                         */
+  int64_t padding_idx;     /* its row gets no gradient; -1: none               */
+  float scale;
+  int grad_output_dtype;   /* fp32, fp16, bf16                                 */
+  int grad_table_dtype;    /* grad_output's dtype or fp32                      */
+  int accumulate;          /* 0: every element of grad_table is written (rows
+                              no id names get zeros); 1: the sums are added to
+                              the rows that ids name, others are not touched   */
+} bevk_embedding_backward_args;
+
+/* Scratch bytes of the backward; 256-byte aligned, needs no initialisation. */
+BEVK_API size_t bevk_embedding_backward_workspace_bytes(const bevk_embedding_backward_args *a);
+/*
+ * grad_table[v, :] (+)= scale * sum over i with ids[i] == v of grad_output[i, :].
+ * The ids are sorted (stably) and each row's sum is taken in fp32 in an order
+ * that the ids alone fix, so equal inputs give equal bits.  Ids outside
+ * [0, num_rows) and padding_idx give no gradient.  num_ids < 2^31 - 2^16.
+ */
+BEVK_API int bevk_embedding_backward(const bevk_embedding_backward_args *a,
+                                     const void *grad_output, const void *ids, void *grad_table,
+                                     void *workspace, size_t workspace_bytes,
+                                     bevk_stream_t stream);
+
 /* One tensor of bevk_grad_clip: numel contiguous elements. */
 typedef struct bevk_grad_tensor {
   const void *grad;

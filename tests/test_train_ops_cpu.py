@@ -7,6 +7,7 @@ import torch
 
 import grad_clip
 import group_norm_act as gna
+import scaled_embedding as emb
 from bevk import cabi
 
 
@@ -118,3 +119,59 @@ def test_grad_clip_checks():
     with pytest.raises(TypeError):
         grad_clip.clip_grad_norm_(3.0, 1.0)
     assert float(grad_clip.clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0)) == 0.0
+
+
+def test_embedding_checks():
+    L = cabi.lib()
+    a = cabi.EmbeddingBackwardArgs()
+
+    def reset(**kw):
+        a.num_ids, a.num_rows, a.dim, a.ids_are_64bit = 10, 20, 8, 1
+        a.grad_output_ld = a.grad_table_ld = 8
+        a.padding_idx, a.scale, a.accumulate = -1, 1.0, 0
+        a.grad_output_dtype = a.grad_table_dtype = cabi.DTYPE_BF16
+        for k, v in kw.items():
+            setattr(a, k, v)
+
+    def call(dy=16, ids=16, out=16, ws=256, nbytes=1 << 30):
+        return L.bevk_embedding_backward(ctypes.byref(a), dy, ids, out, ws, nbytes, None)
+
+    for kw, status in ((dict(grad_output_dtype=cabi.DTYPE_F64), cabi.ERR_UNSUPPORTED),
+                       (dict(grad_table_dtype=cabi.DTYPE_F16), cabi.ERR_UNSUPPORTED),
+                       (dict(num_ids=-1), cabi.ERR_INVALID_ARGUMENT),
+                       (dict(dim=0), cabi.ERR_INVALID_ARGUMENT),
+                       (dict(grad_table_ld=7), cabi.ERR_INVALID_ARGUMENT),
+                       (dict(num_ids=1 << 31), cabi.ERR_INDEX_OVERFLOW),
+                       (dict(num_rows=1 << 31), cabi.ERR_INDEX_OVERFLOW)):
+        reset(**kw)
+        assert L.bevk_embedding_backward_workspace_bytes(ctypes.byref(a)) == 0
+        assert call() == status, kw
+    reset()
+    assert L.bevk_embedding_backward_workspace_bytes(ctypes.byref(a)) > 0
+    assert call(dy=None) == cabi.ERR_INVALID_ARGUMENT
+    assert call(out=None) == cabi.ERR_INVALID_ARGUMENT
+    assert call(nbytes=64) == cabi.ERR_WORKSPACE
+    assert call(ws=128) == cabi.ERR_MISALIGNED
+    reset(num_rows=0)
+    assert call(out=None) == cabi.OK
+    reset(num_ids=0, accumulate=1)
+    assert call(dy=None, ids=None, ws=None, nbytes=0) == cabi.OK
+
+    def look(ld=8, n=4, rows=20, dim=8, dtype=cabi.DTYPE_F32, ids=16):
+        return L.bevk_embedding_forward(16, ld, ids, 1, n, rows, dim, 1.0, 16, dtype, None)
+
+    assert look(dtype=cabi.DTYPE_F64) == cabi.ERR_UNSUPPORTED
+    assert look(n=-1) == cabi.ERR_INVALID_ARGUMENT and look(dim=0) == cabi.ERR_INVALID_ARGUMENT
+    assert look(ids=None) == cabi.ERR_INVALID_ARGUMENT
+    assert look(n=0) == cabi.OK
+
+
+def test_embedding_module_and_no_cpu_fallback():
+    m = emb.ScaledEmbedding(10, 4, padding_idx=-1, scale=2.0)
+    assert set(m.state_dict()) == {"weight"} and not m.weight[9].any() and "scale=2.0" in repr(m)
+    with pytest.raises(ValueError, match="padding_idx"):
+        emb.ScaledEmbedding(10, 4, padding_idx=10)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        m(torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        emb.scaled_embedding_backward(torch.zeros(3, 4), torch.zeros(3, dtype=torch.int64), 10)
