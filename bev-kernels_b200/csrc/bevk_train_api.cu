@@ -38,6 +38,8 @@ int check_group_norm(const bevk_group_norm_problem *p, bool backward) {
   if (p->pixels >= (int64_t(1) << 31) - (1 << 20))
     return fail(BEVK_ERR_INDEX_OVERFLOW, "group_norm_act: %lld pixels exceed 31-bit indexing",
                 static_cast<long long>(p->pixels));
+  if (static_cast<int64_t>(p->batch) * p->channels >= int64_t(1) << 31)
+    return fail(BEVK_ERR_INDEX_OVERFLOW, "group_norm_act: batch x channels exceed 31-bit indexing");
   for (int i = 0; i < 2; ++i)
     if (p->input_strides[i] < 0 || p->output_strides[i] < 0 ||
         (backward && p->grad_output_strides[i] < 0))

@@ -250,20 +250,32 @@ struct SumParams {
   int accumulate;
 };
 
-// The finished sums of VEC columns.
+// The finished sums of VEC columns, 16 bytes of the output at a time.
 template <typename O, int VEC>
-__device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c, float (&v)[VEC]) {
+__device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
+                                       const float (&v)[VEC]) {
+  constexpr int P = VEC < vio::Full<O>::value ? VEC : vio::Full<O>::value;
   O *dst = static_cast<O *>(p.out) + static_cast<int64_t>(row) * p.out_ld + c;
+  float old[VEC];
   if (p.accumulate) {
-    float old[VEC];
-    vio::unpack(vio::load_pack<O, VEC>(dst), old);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = fmaf(v[e], p.scale, old[e]);
+    for (int k = 0; k < VEC; k += P) {
+      float f[P];
+      vio::unpack(vio::load_pack<O, P>(dst + k), f);
+#pragma unroll
+      for (int e = 0; e < P; ++e) old[k + e] = f[e];
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] *= p.scale;
+    for (int e = 0; e < VEC; ++e) old[e] = 0.f;
   }
-  vio::store<O, VEC>(dst, v);
+#pragma unroll
+  for (int k = 0; k < VEC; k += P) {
+    float f[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) f[e] = fmaf(v[k + e], p.scale, old[k + e]);
+    vio::store<O, P>(dst + k, f);
+  }
 }
 
 constexpr int kSumThreads = 256;
@@ -531,8 +543,9 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
 template <typename T, typename O>
 int sum_any(const SumParams &p, int64_t tiles, cudaStream_t stream) {
   constexpr int V = vio::Full<T>::value;
-  const bool vectors = p.dim % V == 0 && p.dy_ld % V == 0 && p.out_ld % V == 0 &&
-                       aligned(p.dy, 16) && aligned(p.out, V * sizeof(O));
+  const bool vectors = p.dim % V == 0 && p.dy_ld % V == 0 &&
+                       p.out_ld * sizeof(O) % 16 == 0 &&
+                       aligned(p.dy, 16) && aligned(p.out, 16);
   return vectors ? sum<T, O, V>(p, tiles, stream) : sum<T, O, 1>(p, tiles, stream);
 }
 

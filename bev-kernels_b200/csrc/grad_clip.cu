@@ -94,14 +94,18 @@ __device__ __forceinline__ float norm_tile(const T *p, int n, bool inf_norm) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) q[k] = vio::load_pack<T, V>(body + (i + k * kThreads) * V);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 4; ++k) {
+      float f[V];
+      vio::unpack(q[k], f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s.take(e, vio::widen(q[k].v[e]));
+      for (int e = 0; e < V; ++e) s.take(e, f[e]);
+    }
   }
   for (; i < vecs; i += kThreads) {
-    const auto q = vio::load_pack<T, V>(body + i * V);
+    float f[V];
+    vio::unpack(vio::load_pack<T, V>(body + i * V), f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) s.take(e, vio::widen(q.v[e]));
+    for (int e = 0; e < V; ++e) s.take(e, f[e]);
   }
   const int tail = n - head - vecs * V;
   if (tid < tail) s.take(1, vio::widen(body[vecs * V + tid]));

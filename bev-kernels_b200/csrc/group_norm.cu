@@ -17,16 +17,23 @@
 // launch does both sweeps.  Every CTA owns a slab of pixels of one image (all
 // channels where C allows): consecutive threads take consecutive 16-byte
 // channel vectors, so a warp reads whole lines, and a thread keeps the same
-// channels for the whole slab (its weights stay in registers).  After the
-// first sweep each CTA leaves one partial result per group, the grid meets,
-// and each CTA merges the partials of its own images in a fixed order before
-// its second sweep.  Images are taken in waves small enough that the second
-// sweep finds the wave in L2.
+// channels throughout (its weights stay in registers).  After the first sweep
+// each CTA leaves one partial result per group, the grid meets, and each CTA
+// joins the partials of its own image in a fixed order before its second
+// sweep.
 //
-// The variance is not a difference of sums of squares: each thread takes mean
-// and squared deviations of a few pixels at a time in registers, and such
-// (count, mean, M2) triples are merged pairwise all the way up, which holds
-// when the mean is far from zero and when single values are far out.
+// Every thread copies its own vectors to shared memory asynchronously -- all
+// of them at once, without registers, and without synchronising with other
+// threads -- and both sweeps read them there.  Images are taken in waves of
+// what the SMs hold together (28 MB); the copies of the next wave follow the
+// second sweep of this one into the slots that it has done with.  The part of
+// a slab that does not fit is read directly, twice.
+//
+// The variance is not a difference of large sums: a thread sums x - pivot and
+// its square around the mean of its own first values, and the threads' (count,
+// mean, M2) are joined by taking the mean of the means and then the squared
+// deviations from it.  That holds when the mean is far from zero and when
+// single values are far out.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -42,11 +49,12 @@ namespace bevk {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kBatch = 4;  // pixels a thread loads before it uses them
-
-// Waves: both sweeps' tensors of one wave of images stay below this, a good
-// half of the 126 MB L2.
-constexpr int64_t kWaveBytes = int64_t(72) << 20;
+constexpr int kBatch = 8;  // vectors of one asynchronous group, or loaded directly
+constexpr int kPairs = 4;  // the backward's: x and dy
+// Shared memory of a CTA; what the reductions leave of it holds vectors.
+constexpr size_t kSmemBytes = 224 << 10;
+// CTAs of a launch at most (one per SM): the workspace is sized for them.
+constexpr int kMostCtas = 160;
 
 struct GnParams {
   const void *x, *dy, *w, *b;
@@ -58,81 +66,169 @@ struct GnParams {
   int64_t xs[2], os[2], gs[2];
   int N, C, G, K;      // K = C / G
   int HW;
-  int S;               // slabs per image
   int nb;              // channel blocks
   int lanes, R;        // threads across a block's channels, rows of pixels
+  int row_team, row_team_log;  // largest power of two <= R, at most team
+  int team, team_log;  // threads that share a group (a power of two)
   int Gb;              // most groups that a channel block touches
   int wave;            // images per wave
-  int param_dtype, act;
+  int S;               // slabs per image: `longer` of slab + 1 pixels, then of slab
+  int slab, longer;
+  int keep;            // vectors (backward: pairs) per thread held in shared memory
+  int param_dtype, param_vectors;  // whether 16-byte loads fit weight and bias
+  int slab_rows, slab_more;    // slab / R, slab % R
+  int parts;                   // row classes that the channel sums are taken in first
+  float inv_lanes, inv_k, inv_pitch;
   float eps;
 };
 
-struct Moments {
-  float n, mean, m2;
-};
-__device__ __forceinline__ Moments merge(const Moments &a, const Moments &b) {
-  const float n = a.n + b.n;
-  const float f = n > 0.f ? b.n / n : 0.f;
-  const float d = b.mean - a.mean;
-  return {n, a.mean + d * f, a.m2 + b.m2 + d * d * (a.n * f)};
-}
-__device__ __forceinline__ Moments merge_xor(const Moments &a, int mask) {
-  const Moments b = {__shfl_xor_sync(0xffffffffu, a.n, mask),
-                     __shfl_xor_sync(0xffffffffu, a.mean, mask),
-                     __shfl_xor_sync(0xffffffffu, a.m2, mask)};
-  // both lanes of a pair merge in the same order, so they hold equal bits
-  const bool low = (threadIdx.x & mask) == 0;
-  return merge(low ? a : b, low ? b : a);
+// n / d for 0 <= n < 2^24 and inv = 1.f / d: a float quotient is off by one at
+// most.  (The compiler's integer division is several times as long, and these
+// stand in front of the first load.)
+__device__ __forceinline__ int quotient(int n, int d, float inv) {
+  int q = static_cast<int>(static_cast<float>(n) * inv);
+  const int r = n - q * d;
+  if (r < 0) --q;
+  if (r >= d) ++q;
+  return q;
 }
 
-// sigmoid: the fp32 path pays for the accurate exponential, 16-bit results
-// hide the fast one's error (a few ulp of fp32) behind their rounding.
-template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
-  return __fdividef(1.f, 1.f + __expf(-z));
+// 1 / d of a count, and 1 / sqrt(v): the approximation and a Newton step, in
+// place of the exact division and root, which stand on the critical path.
+__device__ __forceinline__ float reciprocal(float d) {
+  const float y = __fdividef(1.f, d);
+  return fmaf(y, fmaf(-d, y, 1.f), y);
 }
+__device__ __forceinline__ float reciprocal_root(float v) {
+  const float y = rsqrtf(v);
+  const float z = fmaf(0.5f * y, fmaf(-v * y, y, 1.f), y);
+  return v > 0.f && z == z ? z : y;  // 0 and infinity have their limits
+}
+
+// Sum over the w neighbouring lanes of a team (w a power of two); all get it.
+__device__ __forceinline__ float team_sum(float v, int w) {
+  for (int m = 1; m < w; m <<= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+__device__ __forceinline__ float exp2_approx(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+
+// 1 / (1 + e^-z).  The special-function unit delivers a quarter of the other
+// units' rate, and with two of its results a value (exponential, reciprocal)
+// it would bound the 16-bit kernels.  So those take the reciprocal of
+// d = 1 + e^-z = 2^E (1 + m) from a guess that is linear in m, which a
+// subtraction from d's bits gives: y d = (1 + m)(2 - m - s) / 2 with the shift
+// s = 5 - sqrt(24) that makes the error the same at m = 0 and in the middle
+// (s / 2 = 5 %).  A third-order step, y (1 + h + h^2) with h = 1 - y d, and a
+// Newton step leave (0.05^3)^2 = 1.7e-8: the parameters' gradients are fp32 sums
+// even where the tensors are not.  fp32 tensors get the hardware's reciprocal,
+// and the rounding of -z log2(e) back to first order (at |z| = 10 that is five
+// times the exponential's own error of 2^-22).  The clamps keep infinity out.
 template <typename T>
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == BEVK_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN stays
-  if (act == BEVK_ACT_SILU) return z * sigmoid<T>(z);
+__device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  const vio::Two t2 = vio::mul2(z, vio::two(-kLog2e));
+  const float2 t = vio::split(t2);
+  if constexpr (sizeof(T) == 4) {
+    const float2 f = vio::split(z);
+    const float lx = fmaf(f.x, -kLog2e, -t.x), ly = fmaf(f.y, -kLog2e, -t.y);
+    float ex = exp2_approx(fminf(t.x, 120.f)), ey = exp2_approx(fminf(t.y, 120.f));
+    ex = fmaf(ex, lx * kLn2, ex);
+    ey = fmaf(ey, ly * kLn2, ey);
+    float sx, sy;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sx) : "f"(1.f + ex));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sy) : "f"(1.f + ey));
+    return vio::two(sx, sy);
+  } else {
+    const float ex = exp2_approx(fminf(t.x, 125.f)), ey = exp2_approx(fminf(t.y, 125.f));
+    const vio::Two one = vio::two(1.f);
+    const vio::Two d = vio::add2(vio::two(ex, ey), one);
+    const float2 df = vio::split(d);
+    constexpr int kGuess = 0x7ef311c3;  // (254 - s) 2^23
+    const vio::Two minus = vio::two(-df.x, -df.y);
+    vio::Two y = vio::two(__int_as_float(kGuess - __float_as_int(df.x)),
+                          __int_as_float(kGuess - __float_as_int(df.y)));
+    const vio::Two h = vio::fma2(minus, y, one);
+    y = vio::fma2(y, vio::fma2(h, h, h), y);
+    return vio::fma2(y, vio::fma2(minus, y, one), y);
+  }
+}
+template <typename T, int ACT>
+__device__ __forceinline__ vio::Two activate(vio::Two z) {
+  if constexpr (ACT == BEVK_ACT_RELU) {
+    const float2 f = vio::split(z);
+    return vio::two(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);  // NaN stays
+  }
+  if constexpr (ACT == BEVK_ACT_SILU) return vio::mul2(z, sigmoid<T>(z));
   return z;
 }
-// act'(z); ReLU's is 0 at 0
-template <typename T>
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act == BEVK_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == BEVK_ACT_SILU) {
-    const float s = sigmoid<T>(z);
-    return s * (1.f + z * (1.f - s));
+// d act'(z); ReLU's slope is 0 at 0
+template <typename T, int ACT>
+__device__ __forceinline__ vio::Two through(vio::Two z, vio::Two d) {
+  if constexpr (ACT == BEVK_ACT_RELU) {
+    const float2 f = vio::split(z), g = vio::split(d);
+    return vio::two(f.x > 0.f ? g.x : 0.f, f.y > 0.f ? g.y : 0.f);
   }
-  return 1.f;
+  if constexpr (ACT == BEVK_ACT_SILU) {
+    const vio::Two s = sigmoid<T>(z);
+    const vio::Two rest = vio::fma2(s, vio::two(-1.f), vio::two(1.f));
+    return vio::mul2(d, vio::fma2(vio::mul2(z, s), rest, s));
+  }
+  return d;
 }
 
-// What a CTA is working on: pixels [p0, p0 + count) of image n.
-struct Unit {
-  int n, s, p0, count;
+// Where a thread stands: the same pixels of every wave's image, the same
+// channels.
+struct Place {
+  int cb, s, image;       // channel block, slab, image within the wave
+  int c0, c, bch;         // the block's first channel, the thread's, the block's count
+  int r, lane;            // row of pixels, lane across the channels
+  int p0, count;          // the slab
+  int whole, more;        // rows < more hold whole + 1 of its pixels, the others whole
+  int mine;               // pixels of this thread
+  int g0, ng;             // groups that the block touches
+  bool active;            // whether the thread has channels
 };
-__device__ __forceinline__ Unit unit_of(const GnParams &p, int64_t u) {
-  const int64_t q = u / p.nb;
-  Unit t;
-  t.n = static_cast<int>(q / p.S);
-  t.s = static_cast<int>(q - static_cast<int64_t>(t.n) * p.S);
-  t.p0 = static_cast<int>(static_cast<int64_t>(p.HW) * t.s / p.S);
-  t.count = static_cast<int>(static_cast<int64_t>(p.HW) * (t.s + 1) / p.S) - t.p0;
-  return t;
-}
 __device__ __forceinline__ int slab_pixels(const GnParams &p, int s) {
-  return static_cast<int>(static_cast<int64_t>(p.HW) * (s + 1) / p.S) -
-         static_cast<int>(static_cast<int64_t>(p.HW) * s / p.S);
+  return p.slab + (s < p.longer ? 1 : 0);
 }
-
-// Largest power of two <= 32 of threads per group that lets `groups` groups
-// share the CTA.
-__device__ __forceinline__ int team_width(int groups) {
-  int w = 32;
-  while (w > 1 && w * groups > kThreads) w >>= 1;
-  return w;
+template <int VEC>
+__device__ __forceinline__ Place place(const GnParams &p) {
+  Place t;
+  int q = blockIdx.x;
+  t.cb = 0;
+  if (p.nb > 1) {
+    t.cb = q % p.nb;
+    q /= p.nb;
+  }
+  t.image = 0;
+  if (p.wave > 1) {
+    t.image = q / p.S;
+    q -= t.image * p.S;
+  }
+  t.s = q;
+  t.r = quotient(threadIdx.x, p.lanes, p.inv_lanes);
+  t.lane = threadIdx.x - t.r * p.lanes;
+  t.c0 = t.cb * p.lanes * VEC;
+  t.c = t.c0 + t.lane * VEC;
+  t.bch = min(p.C - t.c0, p.lanes * VEC);
+  t.active = t.r < p.R && t.c < p.C;
+  t.p0 = t.s * p.slab + min(t.s, p.longer);
+  t.count = slab_pixels(p, t.s);
+  t.whole = p.slab_rows;
+  t.more = p.slab_more + (t.count - p.slab);
+  if (t.more == p.R) {
+    ++t.whole;
+    t.more = 0;
+  }
+  t.mine = t.active ? t.whole + (t.r < t.more ? 1 : 0) : 0;
+  t.g0 = quotient(t.c0, p.K, p.inv_k);
+  t.ng = quotient(t.c0 + t.bch - 1, p.K, p.inv_k) + 1 - t.g0;
+  return t;
 }
 
 // The partials of group g of image n: entry e of [0, count) lies in channel
@@ -143,346 +239,530 @@ struct Partials {
   int g, cb0, bw, count;
 };
 __device__ __forceinline__ Partials partials_of(const GnParams &p, int n, int g, int bw) {
+  if (p.nb == 1) return {p.gpart + (static_cast<int64_t>(n) * p.Gb + g) * p.S, g, 0, bw, p.S};
   const int cb0 = g * p.K / bw, cb1 = ((g + 1) * p.K - 1) / bw;
   return {p.gpart + static_cast<int64_t>(n) * p.nb * p.Gb * p.S, g, cb0, bw,
           (cb1 - cb0 + 1) * p.S};
 }
-__device__ __forceinline__ float2 partial(const GnParams &p, const Partials &q, int e, int *s,
-                                          int *channels) {
-  const int b = e / p.S, cb = q.cb0 + b;
-  *s = e - b * p.S;
+// Entry e, and the number of values behind it.
+__device__ __forceinline__ float2 partial(const GnParams &p, const Partials &q, int e,
+                                          float *values) {
+  if (p.nb == 1) {
+    *values = static_cast<float>(slab_pixels(p, e)) * p.K;
+    return __ldcg(q.base + e);
+  }
+  const int b = e / p.S, cb = q.cb0 + b, s = e - b * p.S;
   const int c0 = cb * q.bw;
-  *channels = min((q.g + 1) * p.K, c0 + q.bw) - max(q.g * p.K, c0);
-  return __ldcg(q.base + (static_cast<int64_t>(cb) * p.Gb + (q.g - c0 / p.K)) * p.S + *s);
+  *values = static_cast<float>(slab_pixels(p, s)) *
+            (min((q.g + 1) * p.K, c0 + q.bw) - max(q.g * p.K, c0));
+  return __ldcg(q.base + (static_cast<int64_t>(cb) * p.Gb + (q.g - c0 / p.K)) * p.S + s);
+}
+__device__ __forceinline__ float2 *partial_slot(const GnParams &p, const Place &t, int n, int gl) {
+  return p.gpart + ((static_cast<int64_t>(n) * p.nb + t.cb) * p.Gb + gl) * p.S + t.s;
 }
 
-// Mean and rstd of the ng groups from g0 on, from the slabs' partials; the
-// threads of a team take the partials in turn.
-__device__ void combine_moments(const GnParams &p, int n, int bw, int g0, int ng, float *s_mean,
+// Mean and rstd of the block's groups from the slabs' (mean, M2): first the
+// mean of the means, then the squared deviations from it.  The threads of a
+// team take the partials in turn and keep the first few in registers, so the
+// loads are in flight together.
+__device__ void combine_moments(const GnParams &p, const Place &t, int n, int bw, float *s_mean,
                                 float *s_rstd, bool write) {
-  const int w = team_width(ng), j = threadIdx.x & (w - 1);
-  for (int base = 0; base < ng; base += kThreads / w) {
-    const int gl = base + threadIdx.x / w;
-    Moments t = {0.f, 0.f, 0.f};
-    if (gl < ng) {
-      const Partials q = partials_of(p, n, g0 + gl, bw);
-      for (int e = j; e < q.count; e += w) {
-        int s, channels;
-        const float2 v = partial(p, q, e, &s, &channels);
-        t = merge(t, {static_cast<float>(slab_pixels(p, s)) * channels, v.x, v.y});
-      }
+  constexpr int kKeep = 10;
+  const int w = p.team, j = threadIdx.x & (w - 1);
+  const float inv = reciprocal(static_cast<float>(p.HW) * p.K);
+  for (int base = 0; base < t.ng; base += kThreads >> p.team_log) {
+    const int gl = base + (threadIdx.x >> p.team_log);
+    const bool on = gl < t.ng;
+    const Partials q = partials_of(p, n, on ? t.g0 + gl : t.g0, bw);
+    float2 v[kKeep];
+    float c[kKeep];
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      v[k] = make_float2(0.f, 0.f);
+      c[k] = 0.f;
+      if (on && j + k * w < q.count) v[k] = partial(p, q, j + k * w, &c[k]);
     }
-    for (int m = 1; m < w; m <<= 1) t = merge_xor(t, m);
-    if (gl < ng && j == 0) {
-      const float rstd = 1.f / sqrtf(t.m2 / t.n + p.eps);
-      s_mean[gl] = t.mean;
+    float sum = 0.f, m2 = 0.f, u;
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) sum += c[k] * v[k].x;
+    for (int e = j + kKeep * w; on && e < q.count; e += w) sum += partial(p, q, e, &u).x * u;
+    const float mean = team_sum(sum, w) * inv;
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) m2 += v[k].y + c[k] * (v[k].x - mean) * (v[k].x - mean);
+    for (int e = j + kKeep * w; on && e < q.count; e += w) {
+      const float2 f = partial(p, q, e, &u);
+      m2 += f.y + u * (f.x - mean) * (f.x - mean);
+    }
+    m2 = team_sum(m2, w);
+    if (on && j == 0) {
+      const float rstd = reciprocal_root(fmaf(m2, inv, p.eps));
+      s_mean[gl] = mean;
       s_rstd[gl] = rstd;
       if (write) {
-        p.mean[static_cast<int64_t>(n) * p.G + g0 + gl] = t.mean;
-        p.rstd[static_cast<int64_t>(n) * p.G + g0 + gl] = rstd;
+        p.mean[static_cast<int64_t>(n) * p.G + t.g0 + gl] = mean;
+        p.rstd[static_cast<int64_t>(n) * p.G + t.g0 + gl] = rstd;
       }
     }
   }
 }
 
-template <typename T, int VEC, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) gn_forward_kernel(const __grid_constant__ GnParams p) {
+// The sums' counterpart for the backward.
+__device__ void combine_sums(const GnParams &p, const Place &t, int n, int bw, float inv_m,
+                             float2 *s_sum) {
+  const int w = p.team, j = threadIdx.x & (w - 1);
+  for (int base = 0; base < t.ng; base += kThreads >> p.team_log) {
+    const int gl = base + (threadIdx.x >> p.team_log);
+    float a = 0.f, b = 0.f;
+    if (gl < t.ng) {
+      const Partials q = partials_of(p, n, t.g0 + gl, bw);
+      float u;
+#pragma unroll 10
+      for (int e = j; e < q.count; e += w) {
+        const float2 v = partial(p, q, e, &u);
+        a += v.x;
+        b += v.y;
+      }
+    }
+    a = team_sum(a, w);
+    b = team_sum(b, w);
+    if (gl < t.ng && j == 0) s_sum[gl] = make_float2(a * inv_m, b * inv_m);
+  }
+}
+
+// Whether a vector goes to shared memory by asynchronous 16-byte copies (else
+// through registers).
+template <typename T, int VEC>
+constexpr bool kAsync = sizeof(T) * VEC == 16;
+
+template <typename T, int VEC>
+__device__ __forceinline__ void fetch(char *slot, const T *src) {
+  if constexpr (kAsync<T, VEC>) vio::copy_async16(slot, src);
+  else vio::store_pack<T, VEC>(slot, vio::load_pack<T, VEC>(src));
+}
+
+template <typename T, int VEC, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kThreads, 1) gn_forward_kernel(const __grid_constant__ GnParams p) {
   // statistics columns of a thread: one where its vector lies in one group,
   // else one per channel
   constexpr int NC = WHOLE ? 1 : VEC;
   constexpr int CH = VEC / NC;
-  extern __shared__ float s_dyn[];
-  float2 *s_red = reinterpret_cast<float2 *>(s_dyn);  // [R][lanes * NC]
-  float *s_mean = s_dyn + 2 * kThreads * NC;          // [Gb]
-  float *s_rstd = s_mean + p.Gb;
+  constexpr int kBytes = sizeof(T) * VEC;
+  using Vec = vio::Pack<T, VEC>;
+  extern __shared__ float4 s_dyn[];
+  const int tid = threadIdx.x;
+  char *s_mine = reinterpret_cast<char *>(s_dyn) + tid * kBytes;  // [keep][kThreads] vectors
+  constexpr int kSlot = kThreads * kBytes;
+  float2 *s_red = reinterpret_cast<float2 *>(reinterpret_cast<char *>(s_dyn) + p.keep * kSlot);
+  float *s_mean = reinterpret_cast<float *>(s_red + (kThreads + p.lanes) * NC);
+  float *s_rstd = s_mean + p.Gb;  // [Gb] each
   cg::grid_group grid = cg::this_grid();
 
-  const int tid = threadIdx.x;
-  const int r = tid / p.lanes, lane = tid - r * p.lanes;
-  const int cb = blockIdx.x % p.nb;
-  const int c0 = cb * p.lanes * VEC;
-  const int c = c0 + lane * VEC;
-  const bool active = r < p.R && c < p.C;
-  const int bch = min(p.C - c0, p.lanes * VEC);  // channels of this block
-  const int g0 = c0 / p.K, ng = (c0 + bch - 1) / p.K + 1 - g0;
-  const T *x = static_cast<const T *>(p.x);
-  T *y = static_cast<T *>(p.out);
+  const Place t = place<VEC>(p);
+  const int held = min(t.mine, p.keep);
+  const int groups = (p.keep + kBatch - 1) / kBatch;  // asynchronous ones, of every thread
+  const int64_t hop = static_cast<int64_t>(p.R) * p.xs[1], out_hop = static_cast<int64_t>(p.R) * p.os[1];
+  int n = t.image;
+  const T *src = static_cast<const T *>(p.x) + n * p.xs[0] +
+                 static_cast<int64_t>(t.p0 + t.r) * p.xs[1] + t.c;
+  T *dst = static_cast<T *>(p.out) + n * p.os[0] + static_cast<int64_t>(t.p0 + t.r) * p.os[1] + t.c;
+  for (int g = 0; g < groups; ++g) {
+    for (int i = g * kBatch; i < min(held, (g + 1) * kBatch) && n < p.N; ++i)
+      fetch<T, VEC>(s_mine + i * kSlot, src + i * hop);
+    vio::copy_commit();
+  }
 
   for (int n0 = 0; n0 < p.N; n0 += p.wave) {
-    const int64_t u0 = static_cast<int64_t>(n0) * p.S * p.nb;
-    const int64_t u1 = static_cast<int64_t>(min(p.N, n0 + p.wave)) * p.S * p.nb;
-    for (int64_t u = u0 + blockIdx.x; u < u1; u += gridDim.x) {
-      const Unit t = unit_of(p, u);
-      Moments acc[NC];
+    if (n < p.N) {
+      // sums of x - pivot and its square, the two values of a pair apart; the
+      // pivot is the mean of the first group
+      constexpr int P = vio::kPairsOf<VEC>;
+      float pivot[NC];
+      vio::Two minus[NC == 1 ? 1 : P], sum2[NC == 1 ? 1 : P], sq2[NC == 1 ? 1 : P];
 #pragma unroll
-      for (int k = 0; k < NC; ++k) acc[k] = {0.f, 0.f, 0.f};
-      if (active) {
-        const T *src = x + t.n * p.xs[0] + t.p0 * p.xs[1] + c;
-        int q = r;
-        for (; q + (kBatch - 1) * p.R < t.count; q += kBatch * p.R) {
-          float v[kBatch][VEC];
+      for (int k = 0; k < NC; ++k) pivot[k] = 0.f;
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i)
-            vio::unpack(vio::load_pack<T, VEC>(src + static_cast<int64_t>(q + i * p.R) * p.xs[1]),
-                        v[i]);
+      for (int k = 0; k < (NC == 1 ? 1 : P); ++k) sum2[k] = sq2[k] = vio::two(0.f);
+      const auto aim = [&](const Vec &q) {
+        float f[VEC];
+        vio::unpack(q, f);
 #pragma unroll
-          for (int k = 0; k < NC; ++k) {
-            float sum = 0.f, m2 = 0.f;
+        for (int e = 0; e < VEC; ++e) pivot[e / CH] += f[e];
+      };
+      const auto aimed = [&](float count) {
+        const float inv = reciprocal(count * CH);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i)
+        for (int k = 0; k < NC; ++k) pivot[k] *= inv;
 #pragma unroll
-              for (int e = 0; e < CH; ++e) sum += v[i][k * CH + e];
-            const float mean = sum * (1.f / (kBatch * CH));
+        for (int k = 0; k < (NC == 1 ? 1 : P); ++k)
+          minus[k] = vio::two(-pivot[NC == 1 ? 0 : 2 * k], VEC == 1 ? 0.f : -pivot[NC == 1 ? 0 : 2 * k + 1]);
+      };
+      const auto add = [&](const Vec &q) {
+        vio::Two f[P];
+        vio::unpack2<T, VEC>(q, f);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-              for (int e = 0; e < CH; ++e) {
-                const float d = v[i][k * CH + e] - mean;
-                m2 += d * d;
-              }
-            acc[k] = merge(acc[k], {kBatch * CH, mean, m2});
-          }
+        for (int i = 0; i < P; ++i) {
+          const int k = NC == 1 ? 0 : i;
+          const vio::Two d = vio::add2(f[i], minus[k]);
+          sum2[k] = vio::add2(sum2[k], d);
+          sq2[k] = vio::fma2(d, d, sq2[k]);
         }
-        for (; q < t.count; q += p.R) {
-          float v[VEC];
-          vio::unpack(vio::load_pack<T, VEC>(src + static_cast<int64_t>(q) * p.xs[1]), v);
-#pragma unroll
-          for (int k = 0; k < NC; ++k) {
-            float sum = 0.f, m2 = 0.f;
-#pragma unroll
-            for (int e = 0; e < CH; ++e) sum += v[k * CH + e];
-            const float mean = sum * (1.f / CH);
-#pragma unroll
-            for (int e = 0; e < CH; ++e) {
-              const float d = v[k * CH + e] - mean;
-              m2 += d * d;
-            }
-            acc[k] = merge(acc[k], {CH, mean, m2});
-          }
-        }
-      }
-      const int cols = bch / CH;
-      if (active) {
-#pragma unroll
-        for (int k = 0; k < NC; ++k)
-          s_red[r * cols + lane * NC + k] = make_float2(acc[k].mean, acc[k].m2);
-      }
-      __syncthreads();
-      // one team per group merges the rows and columns of the group
-      const int w = team_width(ng), j = tid & (w - 1);
-      for (int base = 0; base < ng; base += kThreads / w) {
-        const int gl = base + tid / w;
-        Moments m = {0.f, 0.f, 0.f};
-        if (gl < ng) {
-          const int k0 = max((g0 + gl) * p.K - c0, 0) / CH;
-          const int k1 = min((g0 + gl + 1) * p.K - c0, bch) / CH;
-          for (int e = j; e < p.R * (k1 - k0); e += w) {
-            const int row = e / (k1 - k0), col = k0 + e - row * (k1 - k0);
-            if (row >= t.count) break;
-            const float2 v = s_red[row * cols + col];
-            m = merge(m, {static_cast<float>((t.count - row + p.R - 1) / p.R * CH), v.x, v.y});
-          }
-        }
-        for (int k = 1; k < w; k <<= 1) m = merge_xor(m, k);
-        if (gl < ng && j == 0)
-          __stcg(p.gpart + ((static_cast<int64_t>(t.n) * p.nb + cb) * p.Gb + gl) * p.S + t.s,
-                 make_float2(m.mean, m.m2));
-      }
-      __syncthreads();
-    }
-    grid.sync();
-    int have = -1;  // image whose statistics are in shared memory
-    for (int64_t u = u0 + blockIdx.x; u < u1; u += gridDim.x) {
-      const Unit t = unit_of(p, u);
-      if (t.n != have) {
-        __syncthreads();
-        combine_moments(p, t.n, p.lanes * VEC, g0, ng, s_mean, s_rstd,
-                        p.mean != nullptr && t.s == 0);
-        have = t.n;
-        __syncthreads();
-      }
-      if (!active) continue;
-      float mean[VEC], a[VEC], b[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int gl = (c + e) / p.K - g0;
-        mean[e] = s_mean[gl];
-        a[e] = s_rstd[gl] * (p.w ? vio::load_any(p.w, c + e, p.param_dtype) : 1.f);
-        b[e] = p.b ? vio::load_any(p.b, c + e, p.param_dtype) : 0.f;
-      }
-      const T *src = x + t.n * p.xs[0] + t.p0 * p.xs[1] + c;
-      T *dst = y + t.n * p.os[0] + t.p0 * p.os[1] + c;
+      };
+      const auto slot = [&](int i) { return vio::load_pack<T, VEC>(s_mine + i * kSlot); };
+      for (int g = 0; g < groups; ++g) {
+        vio::copy_wait(groups - 1 - g);
+        const int i1 = min(held, (g + 1) * kBatch);
+        if (g == 0) {
 #pragma unroll 4
-      for (int q = r; q < t.count; q += p.R) {
-        float v[VEC];
-        vio::unpack(vio::load_pack<T, VEC>(src + static_cast<int64_t>(q) * p.xs[1]), v);
+          for (int i = 0; i < i1; ++i) aim(slot(i));
+          aimed(static_cast<float>(max(i1, 1)));
+        }
+#pragma unroll 4
+        for (int i = g * kBatch; i < i1; ++i) add(slot(i));
+      }
+      for (int i0 = held; i0 < t.mine; i0 += kBatch) {  // what is not held
+        Vec v[kBatch];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = activate<T>((v[e] - mean[e]) * a[e] + b[e], p.act);
-        vio::store<T, VEC>(dst + static_cast<int64_t>(q) * p.os[1], v);
+        for (int i = 0; i < kBatch; ++i)
+          if (i0 + i < t.mine) v[i] = vio::load_pack<T, VEC>(src + (i0 + i) * hop);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (i0 + i < t.mine) add(v[i]);
+      }
+      // s_red: [statistics column][lane][row], rows padded to an odd number: the
+      // threads of a warp write a row and read a column without bank conflicts
+      const int pitch = p.R | 1;
+      if (t.active) {
+        const float inv = reciprocal(static_cast<float>(max(t.mine, 1) * CH));
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          const float2 s2 = vio::split(sum2[NC == 1 ? 0 : k / 2]), q2 = vio::split(sq2[NC == 1 ? 0 : k / 2]);
+          const float sum = VEC == 1 ? s2.x : NC == 1 ? s2.x + s2.y : k % 2 ? s2.y : s2.x;
+          const float sq = VEC == 1 ? q2.x : NC == 1 ? q2.x + q2.y : k % 2 ? q2.y : q2.x;
+          const float m2 = sq - sum * (sum * inv);
+          s_red[(k * p.lanes + t.lane) * pitch + t.r] =
+              make_float2(pivot[k] + sum * inv, m2 < 0.f ? 0.f : m2);
+        }
+      }
+      __syncthreads();
+      // one team per group joins the rows and columns of the group: the mean
+      // of the means, then the squared deviations from it
+      const int w = p.team, j = tid & (w - 1);
+      const int wr = p.row_team, jr = j & (wr - 1), jc = j >> p.row_team_log;
+      const int wc = w >> p.row_team_log;
+      const int rows = t.whole ? p.R : t.more;
+      for (int base = 0; base < t.ng; base += kThreads >> p.team_log) {
+        const int gl = base + (tid >> p.team_log);
+        int k0 = 0, k1 = 0;
+        if (gl < t.ng) {
+          k0 = max((t.g0 + gl) * p.K - t.c0, 0) / CH;
+          k1 = min((t.g0 + gl + 1) * p.K - t.c0, t.bch) / CH;
+        }
+        const auto at = [&](int row, int k) {  // column k: lane k / NC, entry k % NC
+          return s_red[((k % NC) * p.lanes + k / NC) * pitch + row];
+        };
+        float s = 0.f, m2 = 0.f;
+        for (int row = jr; row < rows; row += wr) {
+          const float c = static_cast<float>((t.whole + (row < t.more ? 1 : 0)) * CH);
+          for (int k = k0 + jc; k < k1; k += wc) s += c * at(row, k).x;
+        }
+        const float mean =
+            team_sum(s, w) * reciprocal(static_cast<float>(t.count) * max((k1 - k0) * CH, 1));
+        for (int row = jr; row < rows; row += wr) {
+          const float c = static_cast<float>((t.whole + (row < t.more ? 1 : 0)) * CH);
+          for (int k = k0 + jc; k < k1; k += wc) {
+            const float2 v = at(row, k);
+            m2 += v.y + c * (v.x - mean) * (v.x - mean);
+          }
+        }
+        m2 = team_sum(m2, w);
+        if (gl < t.ng && j == 0) __stcg(partial_slot(p, t, n, gl), make_float2(mean, m2));
       }
     }
+    const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
+    const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
+    if (p.S > 1 || p.nb > 1) grid.sync();
+    else __syncthreads();
+    const bool next = n + p.wave < p.N;
+    if (n < p.N) {
+      combine_moments(p, t, n, p.lanes * VEC, s_mean, s_rstd, p.mean != nullptr && t.s == 0);
+      __syncthreads();
+      float a[VEC], b[VEC];  // z = a x + b
+      vio::params_to_float(pw, p.w, p.param_dtype, 1.f, a);
+      vio::params_to_float(pb, p.b, p.param_dtype, 0.f, b);
+      if (t.mine > 0) {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          const int gl = quotient(t.c + k * CH, p.K, p.inv_k) - t.g0;
+          const float mean = s_mean[gl], rstd = s_rstd[gl];
+#pragma unroll
+          for (int e = k * CH; e < (k + 1) * CH; ++e) {
+            a[e] *= rstd;
+            b[e] = fmaf(-mean, a[e], b[e]);
+          }
+        }
+      }
+      constexpr int P = vio::kPairsOf<VEC>;
+      vio::Two a2[P], b2[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        a2[i] = VEC == 1 ? vio::two(a[0], 0.f) : vio::two(a[2 * i], a[VEC == 1 ? 0 : 2 * i + 1]);
+        b2[i] = VEC == 1 ? vio::two(b[0], 0.f) : vio::two(b[2 * i], b[VEC == 1 ? 0 : 2 * i + 1]);
+      }
+      const auto write = [&](const Vec &q, int i) {
+        vio::Two v[P];
+        vio::unpack2<T, VEC>(q, v);
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[e] = activate<T, ACT>(vio::fma2(v[e], a2[e], b2[e]));
+        vio::store2<T, VEC>(dst + i * out_hop, v);
+      };
+      const T *src1 = src + p.wave * p.xs[0];
+      for (int g = 0; g < groups; ++g) {
+#pragma unroll 4
+        for (int i = g * kBatch; i < min(held, (g + 1) * kBatch); ++i) {
+          write(vio::load_pack<T, VEC>(s_mine + i * kSlot), i);
+          if (next) fetch<T, VEC>(s_mine + i * kSlot, src1 + i * hop);
+        }
+        vio::copy_commit();
+      }
+#pragma unroll 4
+      for (int i = held; i < t.mine; ++i) write(vio::load_pack<T, VEC>(src + i * hop), i);
+      src = src1;
+      dst += p.wave * p.os[0];
+    }
+    n += p.wave;
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) gn_backward_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float s_dyn[];
-  float2 *s_red = reinterpret_cast<float2 *>(s_dyn);     // [R][lanes * VEC]
-  float2 *s_tot = s_red + kThreads * VEC;                // [lanes * VEC] over all units
-  float2 *s_sum = s_tot + p.lanes * VEC;                 // [Gb] s1 / m, s2 / m
+template <typename T, int VEC, bool WHOLE, int ACT>
+__global__ void __launch_bounds__(kThreads, 1) gn_backward_kernel(const __grid_constant__ GnParams p) {
+  constexpr int NC = WHOLE ? 1 : VEC;  // groups that a thread's vector may touch
+  constexpr int CH = VEC / NC;
+  constexpr int kBytes = sizeof(T) * VEC;
+  using Vec = vio::Pack<T, VEC>;
+  extern __shared__ float4 s_dyn[];
+  const int tid = threadIdx.x;
+  char *s_mine = reinterpret_cast<char *>(s_dyn) + tid * kBytes;  // [keep][x, dy][kThreads]
+  constexpr int kSlot = kThreads * kBytes;
+  float2 *s_red = reinterpret_cast<float2 *>(reinterpret_cast<char *>(s_dyn) + 2 * p.keep * kSlot);
+  float2 *s_tot = s_red + kThreads * VEC;  // s_red: [R][lanes * VEC]; s_tot: over all waves
+  float2 *s_sum = s_tot + p.lanes * VEC;   // [Gb] s1 / m, s2 / m
+  float *s_w = reinterpret_cast<float *>(s_sum + p.Gb);  // [lanes * VEC]
+  // per-channel arrays hold element e of lane l at e * lanes + l
+  const auto entry = [&](int channel) { return channel % VEC * p.lanes + channel / VEC; };
   cg::grid_group grid = cg::this_grid();
 
-  const int tid = threadIdx.x;
-  const int r = tid / p.lanes, lane = tid - r * p.lanes;
-  const int cb = blockIdx.x % p.nb;
-  const int c0 = cb * p.lanes * VEC;
-  const int c = c0 + lane * VEC;
-  const bool active = r < p.R && c < p.C;
-  const int bch = min(p.C - c0, p.lanes * VEC);
-  const int g0 = c0 / p.K, ng = (c0 + bch - 1) / p.K + 1 - g0;
-  const float inv_m = 1.f / (static_cast<float>(p.K) * static_cast<float>(p.HW));
-  const T *x = static_cast<const T *>(p.x);
-  const T *dy = static_cast<const T *>(p.dy);
-  T *dx = static_cast<T *>(p.out);
-
-  for (int k = tid; k < p.lanes * VEC; k += kThreads) s_tot[k] = make_float2(0.f, 0.f);
-  float w[VEC], b[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    w[e] = active && p.w ? vio::load_any(p.w, c + e, p.param_dtype) : 1.f;
-    b[e] = active && p.b ? vio::load_any(p.b, c + e, p.param_dtype) : 0.f;
+  const Place t = place<VEC>(p);
+  const int held = min(t.mine, p.keep);
+  const int groups = (p.keep + kPairs - 1) / kPairs;
+  const int64_t xhop = static_cast<int64_t>(p.R) * p.xs[1];
+  const int64_t ghop = static_cast<int64_t>(p.R) * p.gs[1];
+  const int64_t out_hop = static_cast<int64_t>(p.R) * p.os[1];
+  const int64_t row0 = t.p0 + t.r;
+  int n = t.image;
+  const T *px = static_cast<const T *>(p.x) + n * p.xs[0] + row0 * p.xs[1] + t.c;
+  const T *pg = static_cast<const T *>(p.dy) + n * p.gs[0] + row0 * p.gs[1] + t.c;
+  T *dst = static_cast<T *>(p.out) + n * p.os[0] + row0 * p.os[1] + t.c;
+  for (int g = 0; g < groups; ++g) {
+    for (int i = g * kPairs; i < min(held, (g + 1) * kPairs) && n < p.N; ++i) {
+      fetch<T, VEC>(s_mine + 2 * i * kSlot, px + i * xhop);
+      fetch<T, VEC>(s_mine + (2 * i + 1) * kSlot, pg + i * ghop);
+    }
+    vio::copy_commit();
   }
+  float w[VEC], b[VEC];
+  {
+    const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
+    const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
+    vio::params_to_float(pw, p.w, p.param_dtype, 1.f, w);
+    vio::params_to_float(pb, p.b, p.param_dtype, 0.f, b);
+  }
+  if (t.active && t.r == 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s_w[e * p.lanes + t.lane] = w[e];
+  }
+  constexpr int P = vio::kPairsOf<VEC>;
+  vio::Two w2[P], b2[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    w2[i] = VEC == 1 ? vio::two(w[0], 0.f) : vio::two(w[2 * i], w[VEC == 1 ? 0 : 2 * i + 1]);
+    b2[i] = VEC == 1 ? vio::two(b[0], 0.f) : vio::two(b[2 * i], b[VEC == 1 ? 0 : 2 * i + 1]);
+  }
+  // the pair's groups
+  const auto pair_of = [](const float (&v)[NC], int i) {
+    return NC == 1 ? vio::two(v[0]) : vio::two(v[NC == 1 ? 0 : 2 * i], v[NC == 1 ? 0 : 2 * i + 1]);
+  };
+  int group[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) group[k] = quotient(t.c + k * CH, p.K, p.inv_k);
+  const int pitch = p.lanes * VEC;  // s_red's rows (entries of absent lanes are never used)
+  for (int k = tid; k < pitch; k += kThreads) s_tot[k] = make_float2(0.f, 0.f);
+  const float inv_m = 1.f / (static_cast<float>(p.K) * static_cast<float>(p.HW));
+  const bool params = p.dw != nullptr || p.db != nullptr;
 
   for (int n0 = 0; n0 < p.N; n0 += p.wave) {
-    const int64_t u0 = static_cast<int64_t>(n0) * p.S * p.nb;
-    const int64_t u1 = static_cast<int64_t>(min(p.N, n0 + p.wave)) * p.S * p.nb;
-    for (int64_t u = u0 + blockIdx.x; u < u1; u += gridDim.x) {
-      const Unit t = unit_of(p, u);
-      if (active) {
-        float A[VEC], B[VEC], mean[VEC], rstd[VEC];
+    float rstd[NC], shift[NC];  // xhat = rstd x + shift
+    if (n < p.N) {
+      vio::Two A[P], B[P];
+#pragma unroll
+      for (int e = 0; e < P; ++e) A[e] = B[e] = vio::two(0.f);
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const int64_t g = static_cast<int64_t>(n) * p.G + group[k];
+        rstd[k] = t.active ? p.rstd[g] : 0.f;
+        shift[k] = t.active ? -p.mean[g] * rstd[k] : 0.f;
+      }
+      const auto add = [&](const Vec &qx, const Vec &qg) {
+        vio::Two f[P], d[P];
+        vio::unpack2<T, VEC>(qx, f);
+        vio::unpack2<T, VEC>(qg, d);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const vio::Two xhat = vio::fma2(f[e], pair_of(rstd, e), pair_of(shift, e));
+          const vio::Two dz = through<T, ACT>(vio::fma2(xhat, w2[e], b2[e]), d[e]);
+          A[e] = vio::add2(A[e], dz);
+          B[e] = vio::fma2(dz, xhat, B[e]);
+        }
+      };
+      for (int i0 = held; i0 < t.mine; i0 += kPairs) {
+        Vec qx[kPairs], qg[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          if (i0 + i < t.mine) {
+            qx[i] = vio::load_pack<T, VEC>(px + (i0 + i) * xhop);
+            qg[i] = vio::load_pack<T, VEC>(pg + (i0 + i) * ghop);
+          }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          if (i0 + i < t.mine) add(qx[i], qg[i]);
+      }
+      for (int g = 0; g < groups; ++g) {
+        vio::copy_wait(groups - 1 - g);
+#pragma unroll 2
+        for (int i = g * kPairs; i < min(held, (g + 1) * kPairs); ++i)
+          add(vio::load_pack<T, VEC>(s_mine + 2 * i * kSlot),
+              vio::load_pack<T, VEC>(s_mine + (2 * i + 1) * kSlot));
+      }
+      if (t.active) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          A[e] = B[e] = 0.f;
-          const int64_t g = static_cast<int64_t>(t.n) * p.G + (c + e) / p.K;
-          mean[e] = p.mean[g];
-          rstd[e] = p.rstd[g];
+          const float2 a = vio::split(A[e / 2]), c = vio::split(B[e / 2]);
+          s_red[t.r * pitch + e * p.lanes + t.lane] =
+              e % 2 ? make_float2(a.y, c.y) : make_float2(a.x, c.x);
         }
-        const T *px = x + t.n * p.xs[0] + t.p0 * p.xs[1] + c;
-        const T *pg = dy + t.n * p.gs[0] + t.p0 * p.gs[1] + c;
-#pragma unroll 2
-        for (int q = r; q < t.count; q += p.R) {
-          float v[VEC], d[VEC];
-          vio::unpack(vio::load_pack<T, VEC>(px + static_cast<int64_t>(q) * p.xs[1]), v);
-          vio::unpack(vio::load_pack<T, VEC>(pg + static_cast<int64_t>(q) * p.gs[1]), d);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float xhat = (v[e] - mean[e]) * rstd[e];
-            const float dz = d[e] * slope<T>(xhat * w[e] + b[e], p.act);
-            A[e] += dz;
-            B[e] += dz * xhat;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s_red[r * bch + lane * VEC + e] = make_float2(A[e], B[e]);
       }
       __syncthreads();
-      // channel sums over the rows; row 0 of s_red becomes w * sum
-      for (int k = tid; k < bch; k += kThreads) {
+      // channel sums over the rows, in two steps where threads are left over;
+      // then row 0 of s_red holds w * sum
+      if (p.parts > 1) {
+        const int part = quotient(tid, pitch, p.inv_pitch), k = tid - part * pitch;
+        if (part < p.parts) {
+          float2 s = s_red[part * pitch + k];
+#pragma unroll 4
+          for (int row = part + p.parts; row < p.R; row += p.parts) {
+            const float2 v = s_red[row * pitch + k];
+            s.x += v.x;
+            s.y += v.y;
+          }
+          s_red[part * pitch + k] = s;
+        }
+        __syncthreads();
+      }
+      for (int k = tid; k < pitch; k += kThreads) {
         float2 s = s_red[k];
-        for (int row = 1; row < p.R; ++row) {
-          const float2 v = s_red[row * bch + k];
+#pragma unroll 4
+        for (int row = 1; row < (p.parts > 1 ? p.parts : p.R); ++row) {
+          const float2 v = s_red[row * pitch + k];
           s.x += v.x;
           s.y += v.y;
         }
         s_tot[k].x += s.x;
         s_tot[k].y += s.y;
-        const float wk = p.w ? vio::load_any(p.w, c0 + k, p.param_dtype) : 1.f;
+        const float wk = s_w[k];
         s_red[k] = make_float2(s.x * wk, s.y * wk);
       }
       __syncthreads();
-      const int tw = team_width(ng), j = tid & (tw - 1);
-      for (int base = 0; base < ng; base += kThreads / tw) {
-        const int gl = base + tid / tw;
-        float2 s = make_float2(0.f, 0.f);
-        if (gl < ng) {
-          const int k0 = max((g0 + gl) * p.K - c0, 0), k1 = min((g0 + gl + 1) * p.K - c0, bch);
-          for (int k = k0 + j; k < k1; k += tw) {
-            s.x += s_red[k].x;
-            s.y += s_red[k].y;
+      const int j = tid & (p.team - 1);
+      for (int base = 0; base < t.ng; base += kThreads >> p.team_log) {
+        const int gl = base + (tid >> p.team_log);
+        float s1 = 0.f, s2 = 0.f;
+        if (gl < t.ng) {
+          const int k0 = max((t.g0 + gl) * p.K - t.c0, 0);
+          const int k1 = min((t.g0 + gl + 1) * p.K - t.c0, t.bch);
+          for (int k = k0 + j; k < k1; k += p.team) {
+            const float2 v = s_red[entry(k)];
+            s1 += v.x;
+            s2 += v.y;
           }
         }
-        for (int k = 1; k < tw; k <<= 1) {
-          s.x += __shfl_xor_sync(0xffffffffu, s.x, k);
-          s.y += __shfl_xor_sync(0xffffffffu, s.y, k);
-        }
-        if (gl < ng && j == 0)
-          __stcg(p.gpart + ((static_cast<int64_t>(t.n) * p.nb + cb) * p.Gb + gl) * p.S + t.s, s);
+        s1 = team_sum(s1, p.team);
+        s2 = team_sum(s2, p.team);
+        if (gl < t.ng && j == 0) __stcg(partial_slot(p, t, n, gl), make_float2(s1, s2));
       }
-      __syncthreads();
     }
-    if (n0 + p.wave >= p.N)
-      for (int k = tid; k < bch; k += kThreads)
+    const bool last = n0 + p.wave >= p.N;
+    if (last && params)
+      for (int k = tid; k < pitch; k += kThreads)
         __stcg(p.cpart + static_cast<int64_t>(blockIdx.x) * p.lanes * VEC + k, s_tot[k]);
-    grid.sync();
-    if (p.out != nullptr) {
-      int have = -1;
-      for (int64_t u = u0 + blockIdx.x; u < u1; u += gridDim.x) {
-        const Unit t = unit_of(p, u);
-        if (t.n != have) {
-          __syncthreads();
-          const int tw = team_width(ng), j = tid & (tw - 1);
-          for (int base = 0; base < ng; base += kThreads / tw) {
-            const int gl = base + tid / tw;
-            float2 s = make_float2(0.f, 0.f);
-            if (gl < ng) {
-              const Partials q = partials_of(p, t.n, g0 + gl, p.lanes * VEC);
-              for (int k = j; k < q.count; k += tw) {
-                int slab, channels;
-                const float2 v = partial(p, q, k, &slab, &channels);
-                s.x += v.x;
-                s.y += v.y;
-              }
-            }
-            for (int k = 1; k < tw; k <<= 1) {
-              s.x += __shfl_xor_sync(0xffffffffu, s.x, k);
-              s.y += __shfl_xor_sync(0xffffffffu, s.y, k);
-            }
-            if (gl < ng && j == 0) s_sum[gl] = make_float2(s.x * inv_m, s.y * inv_m);
-          }
-          have = t.n;
-          __syncthreads();
-        }
-        if (!active) continue;
-        float mean[VEC], rstd[VEC];
-        float2 sum[VEC];
+    if (p.S > 1 || p.nb > 1 || (last && params)) grid.sync();
+    else __syncthreads();
+    const bool next = n + p.wave < p.N;
+    if (n < p.N) {
+      const T *px1 = px + p.wave * p.xs[0], *pg1 = pg + p.wave * p.gs[0];
+      if (p.out != nullptr) {
+        combine_sums(p, t, n, p.lanes * VEC, inv_m, s_sum);
+        __syncthreads();
+        float r1[NC], r2[NC];  // dx = rstd w dz + r2 xhat + r1
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int g = (c + e) / p.K;
-          mean[e] = p.mean[static_cast<int64_t>(t.n) * p.G + g];
-          rstd[e] = p.rstd[static_cast<int64_t>(t.n) * p.G + g];
-          sum[e] = s_sum[g - g0];
+        for (int k = 0; k < NC; ++k) {
+          const float2 s = t.active ? s_sum[group[k] - t.g0] : make_float2(0.f, 0.f);
+          r1[k] = -rstd[k] * s.x;
+          r2[k] = -rstd[k] * s.y;
         }
-        const T *px = x + t.n * p.xs[0] + t.p0 * p.xs[1] + c;
-        const T *pg = dy + t.n * p.gs[0] + t.p0 * p.gs[1] + c;
-        T *dst = dx + t.n * p.os[0] + t.p0 * p.os[1] + c;
+        const auto write = [&](const Vec &qx, const Vec &qg, int i) {
+          vio::Two f[P], d[P];
+          vio::unpack2<T, VEC>(qx, f);
+          vio::unpack2<T, VEC>(qg, d);
+#pragma unroll
+          for (int e = 0; e < P; ++e) {
+            const vio::Two xhat = vio::fma2(f[e], pair_of(rstd, e), pair_of(shift, e));
+            const vio::Two dz = through<T, ACT>(vio::fma2(xhat, w2[e], b2[e]), d[e]);
+            f[e] = vio::fma2(vio::mul2(pair_of(rstd, e), w2[e]), dz,
+                             vio::fma2(xhat, pair_of(r2, e), pair_of(r1, e)));
+          }
+          vio::store2<T, VEC>(dst + i * out_hop, f);
+        };
+        for (int g = 0; g < groups; ++g) {
 #pragma unroll 2
-        for (int q = r; q < t.count; q += p.R) {
-          float v[VEC], d[VEC];
-          vio::unpack(vio::load_pack<T, VEC>(px + static_cast<int64_t>(q) * p.xs[1]), v);
-          vio::unpack(vio::load_pack<T, VEC>(pg + static_cast<int64_t>(q) * p.gs[1]), d);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float xhat = (v[e] - mean[e]) * rstd[e];
-            const float dz = d[e] * slope<T>(xhat * w[e] + b[e], p.act);
-            v[e] = rstd[e] * (w[e] * dz - (sum[e].x + xhat * sum[e].y));
+          for (int i = g * kPairs; i < min(held, (g + 1) * kPairs); ++i) {
+            char *slot = s_mine + 2 * i * kSlot;
+            write(vio::load_pack<T, VEC>(slot), vio::load_pack<T, VEC>(slot + kSlot), i);
+            if (next) {
+              fetch<T, VEC>(slot, px1 + i * xhop);
+              fetch<T, VEC>(slot + kSlot, pg1 + i * ghop);
+            }
           }
-          vio::store<T, VEC>(dst + static_cast<int64_t>(q) * p.os[1], v);
+          vio::copy_commit();
+        }
+#pragma unroll 2
+        for (int i = held; i < t.mine; ++i)
+          write(vio::load_pack<T, VEC>(px + i * xhop), vio::load_pack<T, VEC>(pg + i * ghop), i);
+      } else if (next) {
+        for (int g = 0; g < groups; ++g) {
+          for (int i = g * kPairs; i < min(held, (g + 1) * kPairs); ++i) {
+            fetch<T, VEC>(s_mine + 2 * i * kSlot, px1 + i * xhop);
+            fetch<T, VEC>(s_mine + (2 * i + 1) * kSlot, pg1 + i * ghop);
+          }
+          vio::copy_commit();
         }
       }
+      px = px1;
+      pg = pg1;
+      dst += p.wave * p.os[0];
     }
+    n += p.wave;
   }
   // grad_weight and grad_bias: 32 channels at a time, the CTAs' sums in order
-  if (p.dw == nullptr && p.db == nullptr) return;
+  if (!params) return;
   __syncthreads();
   const int wl = tid & 31, wid = tid >> 5;
   const int bw = p.lanes * VEC;
@@ -490,7 +770,8 @@ __global__ void __launch_bounds__(kThreads) gn_backward_kernel(const __grid_cons
     const int ch = base + wl;
     float2 s = make_float2(0.f, 0.f);
     if (ch < p.C) {
-      const int blk = ch / bw, k = ch - blk * bw;
+      const int blk = ch / bw, k = entry(ch - blk * bw);
+#pragma unroll 10
       for (int row = blk + wid * p.nb; row < static_cast<int>(gridDim.x);
            row += (kThreads / 32) * p.nb) {
         const float2 v = __ldcg(p.cpart + static_cast<int64_t>(row) * bw + k);
@@ -501,6 +782,7 @@ __global__ void __launch_bounds__(kThreads) gn_backward_kernel(const __grid_cons
     s_red[wid * 32 + wl] = s;
     __syncthreads();
     if (wid == 0 && ch < p.C) {
+#pragma unroll 5
       for (int k = 1; k < kThreads / 32; ++k) {
         s.x += s_red[k * 32 + wl].x;
         s.y += s_red[k * 32 + wl].y;
@@ -513,29 +795,22 @@ __global__ void __launch_bounds__(kThreads) gn_backward_kernel(const __grid_cons
 }
 
 // CTAs of `kernel` that are resident at once on the current device (0 on an
-// error), remembered per device and shared-memory size.
-template <typename K>
-int resident_ctas(K kernel, size_t smem) {
-  struct Seen {
-    int device = -1;
-    size_t smem = 0;
-    int ctas = 0;
-  };
-  static thread_local Seen seen;
+// error), remembered per kernel and device.
+template <auto kernel>
+int resident_ctas() {
+  static thread_local int seen_device = -1, seen_ctas = 0;
   const int dev = current_device();
   if (dev < 0) return 0;
-  if (seen.device == dev && seen.smem == smem && seen.ctas > 0) return seen.ctas;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem)) != cudaSuccess)
-    return 0;
+  if (seen_device == dev) return seen_ctas;
   int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, smem) !=
-      cudaSuccess)
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(kSmemBytes)) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kSmemBytes) !=
+          cudaSuccess)
     return 0;
-  seen.device = dev;
-  seen.smem = smem;
-  seen.ctas = per_sm * device_info(dev).sm_count;
-  return seen.ctas;
+  seen_ctas = std::min(kMostCtas, per_sm * device_info(dev).sm_count);
+  seen_device = dev;
+  return seen_ctas;
 }
 
 // Channels across the threads of a CTA: everything that follows from the
@@ -551,78 +826,115 @@ void set_lanes(GnParams *p, int vec) {
     const int c0 = cb * p->lanes * vec, c1 = std::min(p->C, c0 + p->lanes * vec);
     p->Gb = std::max(p->Gb, (c1 - 1) / p->K + 1 - c0 / p->K);
   }
+  p->team = 32;
+  p->team_log = 5;
+  while (p->team > 1 && p->team * p->Gb > kThreads) {
+    p->team >>= 1;
+    --p->team_log;
+  }
+  p->row_team = 1;
+  p->row_team_log = 0;
+  while (2 * p->row_team <= std::min(p->R, p->team)) {
+    p->row_team *= 2;
+    ++p->row_team_log;
+  }
+  p->inv_lanes = 1.f / p->lanes;
+  p->inv_k = 1.f / p->K;
+  p->parts = std::min(p->R, std::max(1, kThreads / (p->lanes * vec)));
+  p->inv_pitch = 1.f / (p->lanes * vec);
 }
 
-// Waves and slabs for `ctas` resident CTAs; returns the grid.
-int set_slabs(GnParams *p, int ctas, int64_t image_bytes) {
-  p->wave = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(p->N, kWaveBytes / std::max<int64_t>(image_bytes, 1))));
-  const int64_t per_wave = static_cast<int64_t>(p->wave) * p->nb;
-  // a slab holds at least a batch of pixels for every thread
-  const int64_t most = std::max<int64_t>(1, p->HW / (static_cast<int64_t>(p->R) * kBatch));
-  p->S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas / per_wave, most)));
-  const int64_t grid = std::min<int64_t>(per_wave * p->S, ctas);
-  return static_cast<int>(std::max<int64_t>(p->nb, grid / p->nb * p->nb));
+// Waves and slabs for `ctas` resident CTAs, each with room for `room` vectors
+// of every thread; returns the grid, one CTA per (image of a wave, slab,
+// channel block).  A wave is as many images as the CTAs hold, at least one; the
+// waves are then made equal.
+int set_slabs(GnParams *p, int ctas, int room) {
+  const int64_t image = (p->HW + p->R - 1) / p->R;  // vectors of a thread for a whole image
+  const int64_t most = std::max<int64_t>(
+      1, std::min<int64_t>(ctas / p->nb, ctas * static_cast<int64_t>(room) / (image * p->nb)));
+  const int64_t waves = (p->N + most - 1) / most;
+  p->wave = static_cast<int>((p->N + waves - 1) / waves);
+  // a slab holds at least two pixels for every thread
+  const int64_t cut = std::max<int64_t>(1, p->HW / (static_cast<int64_t>(p->R) * 2));
+  p->S = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(ctas / (static_cast<int64_t>(p->wave) * p->nb), cut)));
+  p->slab = p->HW / p->S;
+  p->longer = p->HW - p->slab * p->S;
+  p->slab_rows = p->slab / p->R;
+  p->slab_more = p->slab - p->slab_rows * p->R;
+  const int slab = p->slab + (p->longer ? 1 : 0);
+  p->keep = std::min(room, (slab + p->R - 1) / p->R);
+  return p->wave * p->nb * p->S;
 }
 
-// An upper bound of the CTAs, for the workspace's size: it must not depend on
-// the device that the size was asked on.
-constexpr int kMostCtas = 148 * 4;
-
-size_t gpart_bytes(const GnParams &p, int S) {
-  return sizeof(float2) * static_cast<size_t>(p.N) * p.nb * p.Gb * S;
+// Bytes of shared memory besides the vectors, and the room that is left.
+size_t reduce_bytes(const GnParams &p, int vec, bool back) {
+  if (back)
+    return sizeof(float2) * (static_cast<size_t>(kThreads) * vec + p.lanes * vec + p.Gb) +
+           sizeof(float) * p.lanes * vec;
+  return sizeof(float2) * ((kThreads + p.lanes) * (p.K % vec == 0 ? 1 : vec) + p.Gb);
+}
+int room_for(size_t reduce, size_t bytes_per_slot) {
+  return static_cast<int>((kSmemBytes - reduce) / (bytes_per_slot * kThreads));
 }
 
-template <typename T, int VEC, bool WHOLE>
-int forward(GnParams p, void *ws, size_t ws_bytes, cudaStream_t stream) {
-  auto kernel = gn_forward_kernel<T, VEC, WHOLE>;
-  const size_t smem = sizeof(float) * (2 * kThreads * (WHOLE ? 1 : VEC) + 2 * p.Gb);
-  const int ctas = std::min(kMostCtas, resident_ctas(kernel, smem));
-  if (ctas < p.nb) return fail(BEVK_ERR_CUDA, "group_norm_act_forward: occupancy query failed");
-  const int grid = set_slabs(&p, ctas, int64_t(2) * p.HW * p.C * sizeof(T));
-  if (ws_bytes < gpart_bytes(p, p.S))
-    return fail(BEVK_ERR_WORKSPACE, "group_norm_act_forward: workspace of %zu bytes, needs %zu",
-                ws_bytes, gpart_bytes(p, p.S));
-  p.gpart = static_cast<float2 *>(ws);
-  void *args[] = {&p};
-  return launched(cudaLaunchCooperativeKernel(reinterpret_cast<void *>(kernel), dim3(grid),
-                                              dim3(kThreads), args, smem, stream),
-                  "gn_forward_kernel");
+size_t gpart_bytes(const GnParams &p) {
+  return sizeof(float2) * static_cast<size_t>(p.N) * p.nb * p.Gb * p.S;
 }
 
-template <typename T, int VEC>
-int backward(GnParams p, void *ws, size_t ws_bytes, cudaStream_t stream) {
-  auto kernel = gn_backward_kernel<T, VEC>;
-  const size_t bw = static_cast<size_t>(p.lanes) * VEC;
-  const size_t smem = sizeof(float2) * (static_cast<size_t>(kThreads) * VEC + bw + p.Gb);
-  const int ctas = std::min(kMostCtas, resident_ctas(kernel, smem));
-  if (ctas < p.nb) return fail(BEVK_ERR_CUDA, "group_norm_act_backward: occupancy query failed");
-  const int grid = set_slabs(&p, ctas, int64_t(3) * p.HW * p.C * sizeof(T));
-  const size_t cbytes = sizeof(float2) * bw * grid;
-  if (ws_bytes < cbytes + gpart_bytes(p, p.S))
-    return fail(BEVK_ERR_WORKSPACE, "group_norm_act_backward: workspace of %zu bytes, needs %zu",
-                ws_bytes, cbytes + gpart_bytes(p, p.S));
+template <auto kernel>
+int launch(GnParams p, int vec, size_t size, bool back, void *ws, size_t ws_bytes,
+           cudaStream_t stream) {
+  const int ctas = resident_ctas<kernel>();
+  if (ctas <= 0) return fail(BEVK_ERR_CUDA, "group_norm_act: occupancy query failed");
+  if (ctas < p.nb)
+    return fail(BEVK_ERR_UNSUPPORTED, "group_norm_act: %d channels are too many", p.C);
+  p.param_vectors = aligned(p.w, 16) && aligned(p.b, 16);
+  const size_t reduce = reduce_bytes(p, vec, back);
+  const size_t slot = (back ? 2 : 1) * vec * size;
+  const int grid = set_slabs(&p, ctas, room_for(reduce, slot));
+  const size_t cpart = back ? static_cast<size_t>(grid) * p.lanes * vec : 0;
+  const size_t need = cpart * sizeof(float2) + gpart_bytes(p);
+  if (ws_bytes < need)
+    return fail(BEVK_ERR_WORKSPACE, "group_norm_act: workspace of %zu bytes, needs %zu", ws_bytes,
+                need);
   p.cpart = static_cast<float2 *>(ws);
-  p.gpart = p.cpart + bw * grid;
+  p.gpart = p.cpart + cpart;
   void *args[] = {&p};
   return launched(cudaLaunchCooperativeKernel(reinterpret_cast<void *>(kernel), dim3(grid),
-                                              dim3(kThreads), args, smem, stream),
-                  "gn_backward_kernel");
+                                              dim3(kThreads), args, reduce + p.keep * slot * kThreads,
+                                              stream),
+                  back ? "gn_backward_kernel" : "gn_forward_kernel");
 }
 
-template <typename T>
+template <typename T, int ACT>
 int dispatch(GnParams &p, bool back, bool vectors, void *ws, size_t ws_bytes,
              cudaStream_t stream) {
   constexpr int V = vio::Full<T>::value;
-  if (vectors) {
-    set_lanes(&p, V);
-    if (back) return backward<T, V>(p, ws, ws_bytes, stream);
-    return p.K % V == 0 ? forward<T, V, true>(p, ws, ws_bytes, stream)
-                        : forward<T, V, false>(p, ws, ws_bytes, stream);
+  const int vec = vectors ? V : 1;
+  set_lanes(&p, vec);
+  const auto run = [&](auto kernel) {
+    return launch<decltype(kernel)::value>(p, vec, sizeof(T), back, ws, ws_bytes, stream);
+  };
+#define BEVK_GN_RUN(...) run(std::integral_constant<void (*)(GnParams), __VA_ARGS__>())
+  if (!vectors)
+    return back ? BEVK_GN_RUN(gn_backward_kernel<T, 1, true, ACT>)
+                : BEVK_GN_RUN(gn_forward_kernel<T, 1, true, ACT>);
+  if (p.K % V == 0)
+    return back ? BEVK_GN_RUN(gn_backward_kernel<T, V, true, ACT>)
+                : BEVK_GN_RUN(gn_forward_kernel<T, V, true, ACT>);
+  return back ? BEVK_GN_RUN(gn_backward_kernel<T, V, false, ACT>)
+              : BEVK_GN_RUN(gn_forward_kernel<T, V, false, ACT>);
+#undef BEVK_GN_RUN
+}
+template <typename T>
+int dispatch(GnParams &p, int act, bool back, bool vectors, void *ws, size_t ws_bytes,
+             cudaStream_t stream) {
+  switch (act) {
+    case BEVK_ACT_RELU: return dispatch<T, BEVK_ACT_RELU>(p, back, vectors, ws, ws_bytes, stream);
+    case BEVK_ACT_SILU: return dispatch<T, BEVK_ACT_SILU>(p, back, vectors, ws, ws_bytes, stream);
+    default: return dispatch<T, BEVK_ACT_NONE>(p, back, vectors, ws, ws_bytes, stream);
   }
-  set_lanes(&p, 1);
-  return back ? backward<T, 1>(p, ws, ws_bytes, stream)
-              : forward<T, 1, true>(p, ws, ws_bytes, stream);
 }
 
 // 16-byte vectors need every pixel of the tensor on a 16-byte boundary.
@@ -643,23 +955,35 @@ GnParams base_params(const bevk_group_norm_problem *q) {
   p.K = q->channels / q->groups;
   p.HW = static_cast<int>(q->pixels);
   p.param_dtype = q->param_dtype;
-  p.act = q->act;
   p.eps = q->eps;
   return p;
+}
+
+int dispatch(const bevk_group_norm_problem *q, GnParams &p, bool back, bool vectors, void *ws,
+             size_t ws_bytes, cudaStream_t stream) {
+  switch (q->dtype) {
+    case BEVK_DTYPE_F16:
+      return dispatch<__half>(p, q->act, back, vectors, ws, ws_bytes, stream);
+    case BEVK_DTYPE_BF16:
+      return dispatch<__nv_bfloat16>(p, q->act, back, vectors, ws, ws_bytes, stream);
+    default: return dispatch<float>(p, q->act, back, vectors, ws, ws_bytes, stream);
+  }
 }
 
 }  // namespace
 
 size_t group_norm_workspace_bytes(const bevk_group_norm_problem *q, bool backward) {
-  // whichever vector width the call takes
+  // whichever vector width the call takes, and however many CTAs it gets: an
+  // image has at most kMostCtas / nb slabs, and a launch kMostCtas CTAs
   size_t most = 0;
-  const int full = static_cast<int>(16 / dtype_size(q->dtype));
-  for (int vec : {1, full}) {
+  const int size = static_cast<int>(dtype_size(q->dtype));
+  for (int vec : {1, 16 / size}) {
     if (q->channels % vec) continue;
     GnParams p = base_params(q);
     set_lanes(&p, vec);
-    set_slabs(&p, kMostCtas, (backward ? 3 : 2) * q->pixels * q->channels * dtype_size(q->dtype));
-    size_t n = gpart_bytes(p, p.S);
+    const int64_t cut = std::max<int64_t>(1, p.HW / (static_cast<int64_t>(p.R) * 2));
+    p.S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostCtas / p.nb, cut)));
+    size_t n = gpart_bytes(p);
     if (backward) n += sizeof(float2) * kMostCtas * static_cast<size_t>(p.lanes) * vec;
     most = std::max(most, n);
   }
@@ -679,11 +1003,7 @@ int launch_group_norm_forward(const bevk_group_norm_problem *q, const void *x, c
   const int64_t size = dtype_size(q->dtype);
   const bool vectors = q->channels * size % 16 == 0 && vector_rows(x, q->input_strides, size) &&
                        vector_rows(y, q->output_strides, size);
-  switch (q->dtype) {
-    case BEVK_DTYPE_F16: return dispatch<__half>(p, false, vectors, ws, ws_bytes, stream);
-    case BEVK_DTYPE_BF16: return dispatch<__nv_bfloat16>(p, false, vectors, ws, ws_bytes, stream);
-    default: return dispatch<float>(p, false, vectors, ws, ws_bytes, stream);
-  }
+  return dispatch(q, p, false, vectors, ws, ws_bytes, stream);
 }
 
 int launch_group_norm_backward(const bevk_group_norm_problem *q, const void *dy, const void *x,
@@ -704,11 +1024,7 @@ int launch_group_norm_backward(const bevk_group_norm_problem *q, const void *dy,
   const bool vectors = q->channels * size % 16 == 0 && vector_rows(x, q->input_strides, size) &&
                        vector_rows(dy, q->grad_output_strides, size) &&
                        (dx == nullptr || vector_rows(dx, q->output_strides, size));
-  switch (q->dtype) {
-    case BEVK_DTYPE_F16: return dispatch<__half>(p, true, vectors, ws, ws_bytes, stream);
-    case BEVK_DTYPE_BF16: return dispatch<__nv_bfloat16>(p, true, vectors, ws, ws_bytes, stream);
-    default: return dispatch<float>(p, true, vectors, ws, ws_bytes, stream);
-  }
+  return dispatch(q, p, true, vectors, ws, ws_bytes, stream);
 }
 
 }  // namespace bevk

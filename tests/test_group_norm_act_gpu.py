@@ -242,6 +242,19 @@ def test_autograd_module_and_differences(cuda):
         assert abs(slope - want) <= 2e-2 * float(gy.norm()), name
 
 
+def test_launches_that_fill_the_device_follow_each_other(cuda):
+    """Each kernel's own limit of resident CTAs decides its launch, whatever ran before it."""
+    for dt, c in ((torch.float32, 256), (torch.float32, 250), (torch.bfloat16, 256),
+                  (torch.float16, 264), (torch.bfloat16, 255)):
+        x, gy, w, b = inputs(12, (2, c, 150, 101), dt, torch.float32, cuda)
+        groups = 1 if c % 8 else 8
+        ref = reference(x, gy, w, b, groups, "silu")
+        y, mean, rstd = gna.group_norm_act_forward(x, groups, w, b, EPS, "silu")
+        check_forward(y, ref, dt)
+        check_backward(gna.group_norm_act_backward(gy, x, mean, rstd, groups, w, b, "silu"), ref,
+                       dt, torch.float32)
+
+
 def test_waves_of_images(cuda):
     """More data than one wave: every image's statistics come from its own pixels."""
     shape = (14, 256, 70, 80)
