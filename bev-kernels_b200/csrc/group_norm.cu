@@ -48,7 +48,10 @@ namespace cg = cooperative_groups;
 namespace bevk {
 namespace {
 
-constexpr int kThreads = 512;
+// Threads of a CTA.  More of them leave each too few registers: 1024 (forward)
+// and 768 (backward) measured 1.2 to 1.5 times the time, with spills.
+constexpr int kForwardThreads = 512;
+constexpr int kBackwardThreads = 512;
 constexpr int kBatch = 8;  // vectors of one asynchronous group, or loaded directly
 constexpr int kPairs = 4;  // the backward's: x and dy
 // Shared memory of a CTA; what the reductions leave of it holds vectors.
@@ -265,6 +268,7 @@ __device__ __forceinline__ float2 *partial_slot(const GnParams &p, const Place &
 // mean of the means, then the squared deviations from it.  The threads of a
 // team take the partials in turn and keep the first few in registers, so the
 // loads are in flight together.
+template <int kThreads>
 __device__ void combine_moments(const GnParams &p, const Place &t, int n, int bw, float *s_mean,
                                 float *s_rstd, bool write) {
   constexpr int kKeep = 10;
@@ -307,25 +311,36 @@ __device__ void combine_moments(const GnParams &p, const Place &t, int n, int bw
 }
 
 // The sums' counterpart for the backward.
+template <int kThreads>
 __device__ void combine_sums(const GnParams &p, const Place &t, int n, int bw, float inv_m,
                              float2 *s_sum) {
+  constexpr int kKeep = 10;
   const int w = p.team, j = threadIdx.x & (w - 1);
   for (int base = 0; base < t.ng; base += kThreads >> p.team_log) {
     const int gl = base + (threadIdx.x >> p.team_log);
+    const bool on = gl < t.ng;
+    const Partials q = partials_of(p, n, on ? t.g0 + gl : t.g0, bw);
+    float2 v[kKeep];
+    float u;
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      v[k] = make_float2(0.f, 0.f);
+      if (on && j + k * w < q.count) v[k] = partial(p, q, j + k * w, &u);
+    }
     float a = 0.f, b = 0.f;
-    if (gl < t.ng) {
-      const Partials q = partials_of(p, n, t.g0 + gl, bw);
-      float u;
-#pragma unroll 10
-      for (int e = j; e < q.count; e += w) {
-        const float2 v = partial(p, q, e, &u);
-        a += v.x;
-        b += v.y;
-      }
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      a += v[k].x;
+      b += v[k].y;
+    }
+    for (int e = j + kKeep * w; on && e < q.count; e += w) {
+      const float2 f = partial(p, q, e, &u);
+      a += f.x;
+      b += f.y;
     }
     a = team_sum(a, w);
     b = team_sum(b, w);
-    if (gl < t.ng && j == 0) s_sum[gl] = make_float2(a * inv_m, b * inv_m);
+    if (on && j == 0) s_sum[gl] = make_float2(a * inv_m, b * inv_m);
   }
 }
 
@@ -341,7 +356,9 @@ __device__ __forceinline__ void fetch(char *slot, const T *src) {
 }
 
 template <typename T, int VEC, bool WHOLE, int ACT>
-__global__ void __launch_bounds__(kThreads, 1) gn_forward_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kForwardThreads, 1)
+    gn_forward_kernel(const __grid_constant__ GnParams p) {
+  constexpr int kThreads = kForwardThreads;
   // statistics columns of a thread: one where its vector lies in one group,
   // else one per channel
   constexpr int NC = WHOLE ? 1 : VEC;
@@ -484,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) gn_forward_kernel(const __grid_co
     else __syncthreads();
     const bool next = n + p.wave < p.N;
     if (n < p.N) {
-      combine_moments(p, t, n, p.lanes * VEC, s_mean, s_rstd, p.mean != nullptr && t.s == 0);
+      combine_moments<kThreads>(p, t, n, p.lanes * VEC, s_mean, s_rstd, p.mean != nullptr && t.s == 0);
       __syncthreads();
       float a[VEC], b[VEC];  // z = a x + b
       vio::params_to_float(pw, p.w, p.param_dtype, 1.f, a);
@@ -534,7 +551,9 @@ __global__ void __launch_bounds__(kThreads, 1) gn_forward_kernel(const __grid_co
 }
 
 template <typename T, int VEC, bool WHOLE, int ACT>
-__global__ void __launch_bounds__(kThreads, 1) gn_backward_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kBackwardThreads, 1)
+    gn_backward_kernel(const __grid_constant__ GnParams p) {
+  constexpr int kThreads = kBackwardThreads;
   constexpr int NC = WHOLE ? 1 : VEC;  // groups that a thread's vector may touch
   constexpr int CH = VEC / NC;
   constexpr int kBytes = sizeof(T) * VEC;
@@ -709,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) gn_backward_kernel(const __grid_c
     if (n < p.N) {
       const T *px1 = px + p.wave * p.xs[0], *pg1 = pg + p.wave * p.gs[0];
       if (p.out != nullptr) {
-        combine_sums(p, t, n, p.lanes * VEC, inv_m, s_sum);
+        combine_sums<kThreads>(p, t, n, p.lanes * VEC, inv_m, s_sum);
         __syncthreads();
         float r1[NC], r2[NC];  // dx = rstd w dz + r2 xhat + r1
 #pragma unroll
@@ -797,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1) gn_backward_kernel(const __grid_c
 // CTAs of `kernel` that are resident at once on the current device (0 on an
 // error), remembered per kernel and device.
 template <auto kernel>
-int resident_ctas() {
+int resident_ctas(int threads) {
   static thread_local int seen_device = -1, seen_ctas = 0;
   const int dev = current_device();
   if (dev < 0) return 0;
@@ -805,7 +824,7 @@ int resident_ctas() {
   int per_sm = 0;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(kSmemBytes)) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kSmemBytes) !=
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, kSmemBytes) !=
           cudaSuccess)
     return 0;
   seen_ctas = std::min(kMostCtas, per_sm * device_info(dev).sm_count);
@@ -813,9 +832,11 @@ int resident_ctas() {
   return seen_ctas;
 }
 
+constexpr int threads_of(bool back) { return back ? kBackwardThreads : kForwardThreads; }
+
 // Channels across the threads of a CTA: everything that follows from the
 // shape, the types and the vector width alone.
-void set_lanes(GnParams *p, int vec) {
+void set_lanes(GnParams *p, int vec, int kThreads) {
   const int total = p->C / vec;
   p->nb = (total + kThreads - 1) / kThreads;
   p->lanes = (total + p->nb - 1) / p->nb;
@@ -869,13 +890,14 @@ int set_slabs(GnParams *p, int ctas, int room) {
 
 // Bytes of shared memory besides the vectors, and the room that is left.
 size_t reduce_bytes(const GnParams &p, int vec, bool back) {
+  const int kThreads = threads_of(back);
   if (back)
     return sizeof(float2) * (static_cast<size_t>(kThreads) * vec + p.lanes * vec + p.Gb) +
            sizeof(float) * p.lanes * vec;
   return sizeof(float2) * ((kThreads + p.lanes) * (p.K % vec == 0 ? 1 : vec) + p.Gb);
 }
-int room_for(size_t reduce, size_t bytes_per_slot) {
-  return static_cast<int>((kSmemBytes - reduce) / (bytes_per_slot * kThreads));
+int room_for(size_t reduce, size_t bytes_per_slot, int threads) {
+  return static_cast<int>((kSmemBytes - reduce) / (bytes_per_slot * threads));
 }
 
 size_t gpart_bytes(const GnParams &p) {
@@ -885,14 +907,15 @@ size_t gpart_bytes(const GnParams &p) {
 template <auto kernel>
 int launch(GnParams p, int vec, size_t size, bool back, void *ws, size_t ws_bytes,
            cudaStream_t stream) {
-  const int ctas = resident_ctas<kernel>();
+  const int threads = threads_of(back);
+  const int ctas = resident_ctas<kernel>(threads);
   if (ctas <= 0) return fail(BEVK_ERR_CUDA, "group_norm_act: occupancy query failed");
   if (ctas < p.nb)
     return fail(BEVK_ERR_UNSUPPORTED, "group_norm_act: %d channels are too many", p.C);
   p.param_vectors = aligned(p.w, 16) && aligned(p.b, 16);
   const size_t reduce = reduce_bytes(p, vec, back);
   const size_t slot = (back ? 2 : 1) * vec * size;
-  const int grid = set_slabs(&p, ctas, room_for(reduce, slot));
+  const int grid = set_slabs(&p, ctas, room_for(reduce, slot, threads));
   const size_t cpart = back ? static_cast<size_t>(grid) * p.lanes * vec : 0;
   const size_t need = cpart * sizeof(float2) + gpart_bytes(p);
   if (ws_bytes < need)
@@ -902,7 +925,7 @@ int launch(GnParams p, int vec, size_t size, bool back, void *ws, size_t ws_byte
   p.gpart = p.cpart + cpart;
   void *args[] = {&p};
   return launched(cudaLaunchCooperativeKernel(reinterpret_cast<void *>(kernel), dim3(grid),
-                                              dim3(kThreads), args, reduce + p.keep * slot * kThreads,
+                                              dim3(threads), args, reduce + p.keep * slot * threads,
                                               stream),
                   back ? "gn_backward_kernel" : "gn_forward_kernel");
 }
@@ -912,7 +935,7 @@ int dispatch(GnParams &p, bool back, bool vectors, void *ws, size_t ws_bytes,
              cudaStream_t stream) {
   constexpr int V = vio::Full<T>::value;
   const int vec = vectors ? V : 1;
-  set_lanes(&p, vec);
+  set_lanes(&p, vec, threads_of(back));
   const auto run = [&](auto kernel) {
     return launch<decltype(kernel)::value>(p, vec, sizeof(T), back, ws, ws_bytes, stream);
   };
@@ -980,7 +1003,7 @@ size_t group_norm_workspace_bytes(const bevk_group_norm_problem *q, bool backwar
   for (int vec : {1, 16 / size}) {
     if (q->channels % vec) continue;
     GnParams p = base_params(q);
-    set_lanes(&p, vec);
+    set_lanes(&p, vec, threads_of(backward));
     const int64_t cut = std::max<int64_t>(1, p.HW / (static_cast<int64_t>(p.R) * 2));
     p.S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostCtas / p.nb, cut)));
     size_t n = gpart_bytes(p);
