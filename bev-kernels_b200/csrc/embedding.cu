@@ -87,23 +87,32 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kDigits = 256;
 constexpr int kMostCluster = 16;
-constexpr int kTile = 32;  // tokens of one tile of the ordered list
+constexpr int kTile = 32;   // tokens of one tile of the ordered list
+constexpr int kShort = 8;   // pieces of a run that one warp joins
 
-struct Owner {  // a run of equal ids that goes on past the tile it begins in
-  unsigned tile, slot;
-};
+using Entry = unsigned long long;  // sort key << 32 | position
+__host__ __device__ constexpr Entry entry_of(unsigned key, unsigned pos) {
+  return static_cast<Entry>(key) << 32 | pos;
+}
+__device__ __forceinline__ unsigned key_in(Entry e) { return static_cast<unsigned>(e >> 32); }
 
 struct SortParams {
   const void *ids;
-  unsigned *key[2], *pos[2];
+  Entry *list[2];
   unsigned *hist;     // [cluster size][kDigits]
-  unsigned *owners;   // how many
-  Owner *owner;
+  // runs of equal ids that go on past the tile they begin in, as 2 * tile + slot
+  // (slot 1: they begin further in than its first token): of at most kShort
+  // pieces, and of more
+  unsigned *count;    // [2]
+  unsigned *owner[2];
   int64_t rows, padding;
   int n, passes, cluster;
-  // zeros of a dense gradient: rows of row_bytes at pitch bytes
-  char *zero;
-  int64_t zero_rows, row_bytes, pitch;
+  int behind_zeros;   // launched while embedding_zero_kernel runs
+};
+
+struct ZeroParams {  // zeros of a dense gradient: rows of row_bytes at pitch bytes
+  char *out;
+  int64_t rows, row_bytes, pitch;
 };
 
 // An id as a sort key; what gets no gradient sorts behind all rows.
@@ -114,135 +123,192 @@ __device__ __forceinline__ unsigned key_of(Id id, const SortParams &p) {
                                                 : static_cast<unsigned>(p.rows);
 }
 
-__device__ void write_zeros(const SortParams &p, int part, int parts) {
-  const int64_t t = static_cast<int64_t>(part) * kSortThreads + threadIdx.x;
-  const int64_t threads = static_cast<int64_t>(parts) * kSortThreads;
+constexpr int kZeroThreads = 512;
+
+// The zeros of a dense gradient, most of its bytes.  The sort needs few SMs and
+// waits for memory most of the time, so it runs at the same time: every CTA
+// here lets it start once the kernels before this one are complete, and the
+// sort waits for this kernel before it ends.
+__global__ void __launch_bounds__(kZeroThreads) embedding_zero_kernel(const ZeroParams p) {
+  ptx::grid_wait_prerequisites();
+  ptx::grid_launch_dependents();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kZeroThreads + threadIdx.x;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kZeroThreads;
   const bool flat = p.row_bytes == p.pitch;
-  const int64_t rows = flat ? 1 : p.zero_rows;
-  const int64_t bytes = flat ? p.zero_rows * p.row_bytes : p.row_bytes;
-  if (reinterpret_cast<uintptr_t>(p.zero) % 16 == 0 && bytes % 16 == 0 &&
+  const int64_t rows = flat ? 1 : p.rows;
+  const int64_t bytes = flat ? p.rows * p.row_bytes : p.row_bytes;
+  if (reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && bytes % 16 == 0 &&
       (flat || p.pitch % 16 == 0)) {
     const int64_t vecs = bytes / 16;
     for (int64_t i = t; i < rows * vecs; i += threads) {
       const int64_t r = flat ? 0 : i / vecs;
-      *reinterpret_cast<uint4 *>(p.zero + r * p.pitch + (i - r * vecs) * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4 *>(p.out + r * p.pitch + (i - r * vecs) * 16) = make_uint4(0, 0, 0, 0);
     }
   } else {  // elements of two bytes at least
     const int64_t halves = bytes / 2;
     for (int64_t i = t; i < rows * halves; i += threads) {
       const int64_t r = flat ? 0 : i / halves;
-      *reinterpret_cast<uint16_t *>(p.zero + r * p.pitch + (i - r * halves) * 2) = 0;
+      *reinterpret_cast<uint16_t *>(p.out + r * p.pitch + (i - r * halves) * 2) = 0;
     }
   }
 }
 
-template <typename Id>
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortParams p) {
-  __shared__ unsigned s_cnt[kSortWarps][kDigits];
-  __shared__ unsigned s_scan[kDigits];
-  ptx::grid_launch_dependents();
-  ptx::grid_wait_prerequisites();
-  if (static_cast<int>(blockIdx.x) >= p.cluster) {
-    write_zeros(p, blockIdx.x - p.cluster, gridDim.x - p.cluster);
-    return;
+// Inclusive sum over the warp's lanes.
+__device__ __forceinline__ unsigned warp_scan(unsigned v) {
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const unsigned u = __shfl_up_sync(0xffffffffu, v, m);
+    if ((threadIdx.x & 31) >= m) v += u;
   }
+  return v;
+}
+
+// Stable least-significant-digit radix sort of (id, position), eight bits a
+// pass.  Every warp owns a stretch of the list.  It counts its digits in order
+// (lanes with equal digits find one another; the first adds them to the warp's
+// own counter), which also ranks every token among the warp's equals; the
+// counters of all warps and CTAs, summed by digit, CTA and warp, say where each
+// goes.  With ITEMS > 0 a thread's tokens stay in registers between the two
+// steps, all loads in flight together; ITEMS = 0 takes any number, reading
+// them twice.
+template <typename Id, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortParams p) {
+  __shared__ alignas(16) unsigned s_cnt[kSortWarps][kDigits];
+  __shared__ unsigned s_warp[kDigits / 32];
+  // behind the zeros everything older is complete already
+  if (!p.behind_zeros) ptx::grid_wait_prerequisites();
   const int rank = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (rank == 0 && tid == 0) *p.owners = 0;
+  if (rank == 0 && tid < 2) p.count[tid] = 0;
   // this CTA's tokens, and this warp's part of them, in order
   const int b0 = static_cast<int>(static_cast<int64_t>(p.n) * rank / p.cluster);
   const int b1 = static_cast<int>(static_cast<int64_t>(p.n) * (rank + 1) / p.cluster);
   const int chunk = ((b1 - b0 + kSortThreads - 1) / kSortThreads) * 32;
   const int w0 = min(b1, b0 + warp * chunk), w1 = min(b1, w0 + chunk);
   const Id *ids = static_cast<const Id *>(p.ids);
+  const auto load = [&](int pass, int i) {
+    return pass ? __ldcg(p.list[(pass + 1) & 1] + i)
+                : entry_of(key_of(ids[i], p), static_cast<unsigned>(i));
+  };
+  // counts a token; returns its rank among the warp's tokens of its digit so far.
+  // Equal digits are found by eight votes: the match instruction takes longer
+  // the more different values the warp holds.
+  const auto tally = [&](bool on, unsigned d) {
+    unsigned same = __ballot_sync(0xffffffffu, on);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const unsigned vote = __ballot_sync(0xffffffffu, (d >> b) & 1u);
+      same &= (d >> b) & 1u ? vote : ~vote;
+    }
+    const unsigned at = on ? s_cnt[warp][d] + __popc(same & ((1u << lane) - 1)) : 0u;
+    __syncwarp();
+    if (on && lane == __ffs(same) - 1) s_cnt[warp][d] += __popc(same);
+    __syncwarp();
+    return at;
+  };
 
   for (int pass = 0; pass < p.passes; ++pass) {
-    const unsigned *kin = p.key[(pass + 1) & 1], *pin = p.pos[(pass + 1) & 1];
-    unsigned *kout = p.key[pass & 1], *pout = p.pos[pass & 1];
-    const int shift = 8 * pass;
-    for (int i = tid; i < kSortWarps * kDigits; i += kSortThreads) (&s_cnt[0][0])[i] = 0;
-    __syncthreads();
-    // digits of the warp's tokens
-    for (int i = w0 + lane; i - lane < w1; i += 32) {
-      const unsigned active = __ballot_sync(0xffffffffu, i < w1);
-      if (i < w1) {
-        const unsigned k = pass ? __ldcg(kin + i) : key_of(ids[i], p);
-        const unsigned d = (k >> shift) & (kDigits - 1);
-        const unsigned same = __match_any_sync(active, d);
-        if (lane == __ffs(same) - 1) s_cnt[warp][d] += __popc(same);
+    Entry *out = p.list[pass & 1];
+    const int shift = 32 + 8 * pass;
+    Entry item[ITEMS > 0 ? ITEMS : 1];
+    unsigned at[ITEMS > 0 ? ITEMS : 1];
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        const int i = w0 + k * 32 + lane;
+        item[k] = i < w1 ? load(pass, i) : 0;
       }
-      __syncwarp();
+    }
+#pragma unroll
+    for (int i = tid; i < kSortWarps * kDigits / 4; i += kSortThreads)
+      reinterpret_cast<uint4 *>(&s_cnt[0][0])[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        at[k] = tally(w0 + k * 32 + lane < w1,
+                      static_cast<unsigned>(item[k] >> shift) & (kDigits - 1));
+    } else {
+      for (int i = w0 + lane; i - lane < w1; i += 32)
+        tally(i < w1, i < w1 ? static_cast<unsigned>(load(pass, i) >> shift) & (kDigits - 1) : 0u);
     }
     __syncthreads();
     // digit totals of the CTA, over the cluster
+    unsigned mine = 0;
     if (tid < kDigits) {
-      unsigned sum = 0;
-      for (int w = 0; w < kSortWarps; ++w) sum += s_cnt[w][tid];
-      __stcg(p.hist + rank * kDigits + tid, sum);
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) mine += s_cnt[w][tid];
+      __stcg(p.hist + rank * kDigits + tid, mine);
     }
     ptx::cluster_sync();
-    unsigned before = 0, total = 0;
+    unsigned before = 0, total = 0, scan = 0;
     if (tid < kDigits) {
-      for (int r = 0; r < p.cluster; ++r) {
-        const unsigned h = __ldcg(p.hist + r * kDigits + tid);
-        if (r < rank) before += h;
-        total += h;
+      unsigned h[kMostCluster];
+#pragma unroll
+      for (int r = 0; r < kMostCluster; ++r)
+        h[r] = r < p.cluster ? __ldcg(p.hist + r * kDigits + tid) : 0;
+#pragma unroll
+      for (int r = 0; r < kMostCluster; ++r) {
+        if (r < rank) before += h[r];
+        total += h[r];
       }
-      s_scan[tid] = total;
+      scan = warp_scan(total);
+      if (lane == 31) s_warp[warp] = scan;
     }
     __syncthreads();
-    for (int m = 1; m < kDigits; m <<= 1) {  // inclusive scan over the digits
-      unsigned v = 0;
-      if (tid < kDigits && tid >= m) v = s_scan[tid - m];
-      __syncthreads();
-      if (tid < kDigits) s_scan[tid] += v;
-      __syncthreads();
-    }
     if (tid < kDigits) {
-      unsigned at = s_scan[tid] - total + before;
+      unsigned first = scan - total + before;
+#pragma unroll
+      for (int w = 0; w < kDigits / 32; ++w)
+        if (w < warp) first += s_warp[w];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
         const unsigned c = s_cnt[w][tid];
-        s_cnt[w][tid] = at;
-        at += c;
+        s_cnt[w][tid] = first;
+        first += c;
       }
     }
     __syncthreads();
-    for (int i = w0 + lane; i - lane < w1; i += 32) {
-      const unsigned active = __ballot_sync(0xffffffffu, i < w1);
-      if (i < w1) {
-        const unsigned k = pass ? __ldcg(kin + i) : key_of(ids[i], p);
-        const unsigned d = (k >> shift) & (kDigits - 1);
-        const unsigned same = __match_any_sync(active, d);
-        const unsigned at = s_cnt[warp][d] + __popc(same & ((1u << lane) - 1));
-        __syncwarp(active);
-        if (lane == __ffs(same) - 1) s_cnt[warp][d] += __popc(same);
-        kout[at] = k;
-        pout[at] = pass ? __ldcg(pin + i) : static_cast<unsigned>(i);
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+        if (w0 + k * 32 + lane < w1)
+          out[s_cnt[warp][static_cast<unsigned>(item[k] >> shift) & (kDigits - 1)] + at[k]] = item[k];
+    } else {
+      for (int i = w0 + lane; i - lane < w1; i += 32) {
+        const Entry e = i < w1 ? load(pass, i) : 0;
+        const unsigned to = tally(i < w1, static_cast<unsigned>(e >> shift) & (kDigits - 1));
+        if (i < w1) out[to] = e;
       }
-      __syncwarp();
     }
     ptx::cluster_sync();
   }
   // runs that go on past the tile they begin in
-  const unsigned *key = p.key[(p.passes + 1) & 1];
+  const Entry *list = p.list[(p.passes + 1) & 1];
   const int tiles = (p.n + kTile - 1) / kTile;
   for (int t = rank * kSortThreads + tid; t < tiles; t += p.cluster * kSortThreads) {
-    const int64_t last = static_cast<int64_t>(t) * kTile + kTile - 1;
-    if (last + 1 >= p.n) continue;
-    const unsigned k = __ldcg(key + last);
-    if (k >= static_cast<unsigned>(p.rows) || __ldcg(key + last + 1) != k) continue;
-    if (t > 0 && __ldcg(key + static_cast<int64_t>(t) * kTile - 1) == k) continue;
-    const unsigned slot = __ldcg(key + static_cast<int64_t>(t) * kTile) == k ? 0u : 1u;
-    p.owner[atomicAdd(p.owners, 1u)] = {static_cast<unsigned>(t), slot};  // any order will do
+    const int64_t first = static_cast<int64_t>(t) * kTile, next = first + kTile;
+    if (next >= p.n) continue;
+    const int64_t far = first + int64_t(kShort) * kTile;  // where a run of more pieces still is
+    const unsigned k = key_in(__ldcg(list + next - 1)), after = key_in(__ldcg(list + next));
+    const unsigned start = key_in(__ldcg(list + first));
+    const unsigned prior = t > 0 ? key_in(__ldcg(list + first - 1)) : ~0u;
+    const unsigned later = far < p.n ? key_in(__ldcg(list + far)) : ~0u;
+    if (k >= static_cast<unsigned>(p.rows) || after != k || prior == k) continue;
+    const int is_long = later == k;
+    // the lists' order changes nothing
+    p.owner[is_long][atomicAdd(p.count + is_long, 1u)] = 2 * t + (start == k ? 0 : 1);
   }
+  ptx::grid_launch_dependents();
+  if (p.behind_zeros) ptx::grid_wait_prerequisites();
 }
 
 // -------------------------------------------------------------------- sums
 struct SumParams {
   const void *dy;
   void *out;
-  const unsigned *key, *pos;
-  const unsigned *owners;
-  const Owner *owner;
+  const Entry *list;
+  const unsigned *count;
+  const unsigned *owner[2];
   float *partial;    // [tile][2][pdim]: a run's piece at the tile's start, or further in
   int64_t dy_ld, out_ld;
   int n, rows, dim, pdim, slices;
@@ -256,6 +322,19 @@ __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
                                        const float (&v)[VEC]) {
   constexpr int P = VEC < vio::Full<O>::value ? VEC : vio::Full<O>::value;
   O *dst = static_cast<O *>(p.out) + static_cast<int64_t>(row) * p.out_ld + c;
+  if constexpr (sizeof(O) == 4 && VEC >= 4) {
+    if (p.accumulate) {
+      // nobody else writes these elements: the addition can be left to L2, and
+      // the warp does not wait for the old values
+#pragma unroll
+      for (int k = 0; k < VEC; k += 4)
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst + k),
+                     "f"(v[k] * p.scale), "f"(v[k + 1] * p.scale), "f"(v[k + 2] * p.scale),
+                     "f"(v[k + 3] * p.scale)
+                     : "memory");
+      return;
+    }
+  }
   float old[VEC];
   if (p.accumulate) {
 #pragma unroll
@@ -279,11 +358,11 @@ __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
 }
 
 constexpr int kSumThreads = 256;
-constexpr int kAhead = 8;  // rows loaded before they are used
+constexpr int kAhead = 16;  // rows loaded before they are used
 
 // One warp per (tile, slice of 32 * VEC columns).
 template <typename T, typename O, int VEC>
-__global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumParams p) {
+__global__ void __launch_bounds__(kSumThreads, 2) embedding_sum_kernel(const SumParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_wait_prerequisites();
   const int lane = threadIdx.x & 31;
@@ -292,13 +371,12 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
   const int c = (static_cast<int>(item - tile * p.slices) * 32 + lane) * VEC;
   const int64_t first = tile * kTile;
   if (first >= p.n) return;
-  const bool have = first + lane < p.n;
-  const unsigned none = static_cast<unsigned>(p.rows);
-  const unsigned key = have ? p.key[first + lane] : none;
-  const unsigned pos = have ? p.pos[first + lane] : 0u;
-  const unsigned before = first > 0 ? p.key[first - 1] : none;
-  const unsigned after = first + kTile < p.n ? p.key[first + kTile] : none;
-  const int count = __popc(__ballot_sync(0xffffffffu, key != none));  // rows come first
+  const Entry none = entry_of(static_cast<unsigned>(p.rows), 0);
+  const Entry e = first + lane < p.n ? p.list[first + lane] : none;
+  const unsigned before = key_in(first > 0 ? p.list[first - 1] : none);
+  const unsigned after = key_in(first + kTile < p.n ? p.list[first + kTile] : none);
+  const unsigned key = key_in(e), pos = static_cast<unsigned>(e);
+  const int count = __popc(__ballot_sync(0xffffffffu, key != key_in(none)));  // rows come first
   const unsigned next = __shfl_down_sync(0xffffffffu, key, 1);
   // bit j: token j is the last of its run within the tile
   const unsigned ends = __ballot_sync(0xffffffffu, lane == 31 || key != next);
@@ -306,7 +384,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
   const bool col = c < p.dim;
   float acc[VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   int begin = 0;
   for (int j0 = 0; j0 < count; j0 += kAhead) {
     vio::Pack<T, VEC> q[kAhead];
@@ -324,7 +402,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
         float v[VEC];
         vio::unpack(q[j], v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
       }
       if ((ends >> t) & 1u) {
         const unsigned row = __shfl_sync(0xffffffffu, key, t);
@@ -332,41 +410,73 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const SumPar
         if (col) {
           if (open) {
             float *dst = p.partial + (tile * 2 + (begin ? 1 : 0)) * p.pdim + c;
+            if constexpr (VEC % 4 == 0) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) __stcg(dst + e, acc[e]);
+              for (int k = 0; k < VEC; k += 4)
+                __stcg(reinterpret_cast<float4 *>(dst + k),
+                       make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]));
+            } else {
+#pragma unroll
+              for (int k = 0; k < VEC; ++k) __stcg(dst + k, acc[k]);
+            }
           } else {
             finish<O, VEC>(p, row, c, acc);
           }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
         begin = t + 1;
       }
     }
   }
 }
 
-// Runs that cross tiles: a CTA adds the pieces of one run for 128 columns,
-// each warp a stretch of them in order, then the warps' sums in order.
+// Writes four columns of a joined run.
 template <typename O>
-__global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumParams p) {
+__device__ __forceinline__ void finish_four(const SumParams &p, unsigned row, int c, float4 s,
+                                            bool vectors) {
+  const float f[4] = {s.x, s.y, s.z, s.w};
+  if (vectors) {
+    if (c < p.dim) finish<O, 4>(p, row, c, f);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float one[1] = {f[k]};
+    if (c + k < p.dim) finish<O, 1>(p, row, c + k, one);
+  }
+}
+__device__ __forceinline__ void add4(float4 *s, const float4 v) {
+  s->x += v.x;
+  s->y += v.y;
+  s->z += v.z;
+  s->w += v.w;
+}
+
+// Runs that cross tiles, 128 columns at a time.  A warp joins a run of few
+// pieces, all loads in flight; a CTA one of many, each warp a stretch of them in
+// order and then the warps' sums in order.
+template <typename O>
+__global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumParams p,
+                                                                     const int vectors) {
   constexpr int kWarps = kSumThreads / 32;
   __shared__ float4 s_sum[kWarps][32];
   ptx::grid_launch_dependents();
   ptx::grid_wait_prerequisites();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slices = (p.pdim + 127) / 128;
-  const int64_t items = static_cast<int64_t>(*p.owners) * slices;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const Owner o = p.owner[item / slices];
+  const int64_t few = static_cast<int64_t>(p.count[0]) * slices;
+  const int64_t many = static_cast<int64_t>(p.count[1]) * slices;
+  for (int64_t item = blockIdx.x; item < many; item += gridDim.x) {
+    const unsigned o = p.owner[1][item / slices];
     const int c = static_cast<int>(item % slices) * 128 + lane * 4;
-    const int64_t first = static_cast<int64_t>(o.tile) * kTile;
-    const unsigned row = p.key[first + kTile - 1];
-    // tiles after o.tile whose first token is still of this run
-    int more = 0;
+    const int64_t tile = o >> 1;
+    const unsigned row = key_in(p.list[tile * kTile + kTile - 1]);
+    // tiles after this one whose first token is still of the run
+    int more = kShort;
     for (;;) {
-      const int64_t t = (o.tile + 1 + static_cast<int64_t>(more) + lane) * kTile;
-      const unsigned on = __ballot_sync(0xffffffffu, t < p.n && p.key[t] == row);
+      const int64_t t = (tile + 1 + more + lane) * kTile;
+      const unsigned on = __ballot_sync(0xffffffffu, t < p.n && key_in(p.list[t]) == row);
       const int run = on == 0xffffffffu ? 32 : __ffs(~on) - 1;
       more += run;
       if (run < 32) break;
@@ -376,37 +486,41 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumPa
     const int a = min(pieces, warp * per), b = min(pieces, a + per);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < p.pdim) {
-      const float *src = p.partial + c;
 #pragma unroll 8
       for (int k = a; k < b; ++k) {
-        const int64_t at = (static_cast<int64_t>(o.tile) + k) * 2 + (k == 0 ? o.slot : 0u);
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + at * p.pdim));
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+        const int64_t at = (tile + k) * 2 + (k == 0 ? o & 1 : 0u);
+        add4(&s, __ldcg(reinterpret_cast<const float4 *>(p.partial + at * p.pdim + c)));
       }
     }
     s_sum[warp][lane] = s;
     __syncthreads();
     if (warp == 0) {
-      for (int w = 1; w < kWarps; ++w) {
-        const float4 v = s_sum[w][lane];
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
-      }
-      const float f[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (c + e < p.dim) {
-          float one[1] = {f[e]};
-          finish<O, 1>(p, row, c + e, one);
-        }
-      }
+      for (int w = 1; w < kWarps; ++w) add4(&s, s_sum[w][lane]);
+      finish_four<O>(p, row, c, s, vectors != 0);
     }
     __syncthreads();
+  }
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + warp; item < few;
+       item += static_cast<int64_t>(gridDim.x) * kWarps) {
+    const unsigned o = p.owner[0][item / slices];
+    const int c = static_cast<int>(item % slices) * 128 + lane * 4;
+    const int64_t tile = o >> 1;
+    // lane k >= 1: whether the run still is at tile + k; the row from lane 0
+    const int64_t t = lane == 0 ? tile * kTile + kTile - 1 : (tile + lane) * kTile;
+    const unsigned key = lane < kShort && t < p.n ? key_in(p.list[t]) : ~0u;
+    const unsigned row = __shfl_sync(0xffffffffu, key, 0);
+    const int pieces = __ffs(~__ballot_sync(0xffffffffu, key == row)) - 1;
+    if (c >= p.pdim) continue;
+    float4 v[kShort], s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kShort; ++k) {
+      const int64_t at = (tile + k) * 2 + (k == 0 ? o & 1 : 0u);
+      if (k < pieces) v[k] = __ldcg(reinterpret_cast<const float4 *>(p.partial + at * p.pdim + c));
+    }
+#pragma unroll
+    for (int k = 0; k < kShort; ++k)
+      if (k < pieces) add4(&s, v[k]);
+    finish_four<O>(p, row, c, s, vectors != 0);
   }
 }
 
@@ -436,7 +550,7 @@ int look_any(const LookParams &p, bool wide_ids, cudaStream_t stream) {
 }
 
 struct Layout {  // of the backward's workspace
-  size_t key[2], pos[2], hist, owners, owner, partial, bytes;
+  size_t list[2], hist, count, owner[2], partial, bytes;
   int64_t tiles;
   int pdim;
 };
@@ -452,32 +566,30 @@ Layout layout_of(const bevk_embedding_backward_args *a) {
   l.tiles = (a->num_ids + kTile - 1) / kTile;
   l.pdim = (a->dim + 3) / 4 * 4;
   for (int i = 0; i < 2; ++i) {
-    l.key[i] = take(n * 4);
-    l.pos[i] = take(n * 4);
+    l.list[i] = take(n * sizeof(Entry));
+    l.owner[i] = take(sizeof(unsigned) * static_cast<size_t>(l.tiles));
   }
   l.hist = take(sizeof(unsigned) * kMostCluster * kDigits);
-  l.owners = take(sizeof(unsigned));
-  l.owner = take(sizeof(Owner) * static_cast<size_t>(l.tiles));
+  l.count = take(2 * sizeof(unsigned));
   l.partial = take(sizeof(float) * 2 * static_cast<size_t>(l.tiles) * l.pdim);
   l.bytes = at;
   return l;
 }
 
-// CTAs of the sorting cluster: 4096 tokens each up to the hardware's most
-// (16 where a cluster of that size fits on the device, else 8).
+// CTAs of the sorting cluster: a token a thread, up to the hardware's most (16
+// where a cluster of that size fits on the device, else 8).
 int cluster_size(int64_t n) {
   int c = 1;
-  while (c < kMostCluster && n > int64_t(4096) * c) c <<= 1;
+  while (c < kMostCluster && n > int64_t(kSortThreads) * c) c <<= 1;
   return c;
 }
 
-template <typename Id>
-int sort_ids(const SortParams &p0, bool dense, cudaStream_t stream) {
+template <auto kernel>
+int sort_ids(const SortParams &p0, int cluster, cudaStream_t stream) {
   SortParams p = p0;
   const int dev = current_device();
   if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
-  auto kernel = embedding_sort_kernel<Id>;
-  p.cluster = cluster_size(p.n);
+  p.cluster = cluster;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -506,16 +618,24 @@ int sort_ids(const SortParams &p0, bool dense, cudaStream_t stream) {
     }
     if (fits < 1) attr[0].val.clusterDim.x = p.cluster = 8;
   }
-  int grid = p.cluster;
-  if (dense) {  // about an SM's worth of CTAs for every other SM, in whole clusters
-    const int64_t bytes = p.zero_rows * p.row_bytes;
-    const int64_t want = std::max<int64_t>(1, bytes / (64 * kSortThreads));
-    const int64_t room = std::max(1, device_info(dev).sm_count - p.cluster);
-    const int extra = static_cast<int>(std::min(want, room));
-    grid += (extra + p.cluster - 1) / p.cluster * p.cluster;
-  }
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(p.cluster);
   return launched(cudaLaunchKernelEx(&cfg, kernel, p), "embedding_sort_kernel");
+}
+
+// Picks the tokens that a thread keeps in registers.
+template <typename Id>
+int sort_any(const SortParams &p, cudaStream_t stream) {
+  const int cluster = cluster_size(p.n);
+  // the half-sized cluster of a device without room for 16 CTAs holds twice as many each
+  const int64_t each = (p.n + cluster - 1) / cluster * (cluster > 8 ? 2 : 1);
+  if (each <= kSortThreads) return sort_ids<embedding_sort_kernel<Id, 1>>(p, cluster, stream);
+  if (each <= 2 * kSortThreads)
+    return sort_ids<embedding_sort_kernel<Id, 2>>(p, cluster, stream);
+  if (each <= 4 * kSortThreads)
+    return sort_ids<embedding_sort_kernel<Id, 4>>(p, cluster, stream);
+  if (each <= 8 * kSortThreads)
+    return sort_ids<embedding_sort_kernel<Id, 8>>(p, cluster, stream);
+  return sort_ids<embedding_sort_kernel<Id, 0>>(p, cluster, stream);
 }
 
 template <typename T, typename O, int VEC>
@@ -533,10 +653,11 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
   if (st != BEVK_OK) return st;
   if (tiles < 2) return BEVK_OK;  // no run crosses tiles
   const int64_t items = (tiles - 1) * ((p.pdim + 127) / 128);
-  const int64_t most = int64_t(4) * device_info(current_device()).sm_count;
+  const int64_t most = int64_t(8) * device_info(current_device()).sm_count;
+  const int vectors = p.dim % 4 == 0 && p.out_ld * sizeof(O) % 16 == 0 && aligned(p.out, 16);
   return launched(launch_dependent(embedding_join_kernel<O>,
                                    dim3(static_cast<unsigned>(std::min(items, most))),
-                                   dim3(kSumThreads), 0, stream, p),
+                                   dim3(kSumThreads), 0, stream, p, vectors),
                   "embedding_join_kernel");
 }
 
@@ -573,32 +694,40 @@ int launch_embedding_backward(const bevk_embedding_backward_args *a, const void 
   SortParams s = {};
   s.ids = ids;
   for (int i = 0; i < 2; ++i) {
-    s.key[i] = reinterpret_cast<unsigned *>(base + l.key[i]);
-    s.pos[i] = reinterpret_cast<unsigned *>(base + l.pos[i]);
+    s.list[i] = reinterpret_cast<Entry *>(base + l.list[i]);
+    s.owner[i] = reinterpret_cast<unsigned *>(base + l.owner[i]);
   }
   s.hist = reinterpret_cast<unsigned *>(base + l.hist);
-  s.owners = reinterpret_cast<unsigned *>(base + l.owners);
-  s.owner = reinterpret_cast<Owner *>(base + l.owner);
+  s.count = reinterpret_cast<unsigned *>(base + l.count);
   s.rows = a->num_rows;
   s.padding = a->padding_idx;
   s.n = static_cast<int>(a->num_ids);
   s.passes = 1;
   while (s.passes < 4 && (a->num_rows >> (8 * s.passes)) != 0) ++s.passes;
-  const int64_t size = dtype_size(a->grad_table_dtype);
-  s.zero = static_cast<char *>(grad_table);
-  s.zero_rows = a->num_rows;
-  s.row_bytes = a->dim * size;
-  s.pitch = a->grad_table_ld * size;
-  const int st = a->ids_are_64bit ? sort_ids<int64_t>(s, !a->accumulate, stream)
-                                  : sort_ids<int32_t>(s, !a->accumulate, stream);
+  int st = BEVK_OK;
+  if (!a->accumulate) {
+    const int64_t size = dtype_size(a->grad_table_dtype);
+    const ZeroParams z = {static_cast<char *>(grad_table), a->num_rows, a->dim * size,
+                          a->grad_table_ld * size};
+    const int64_t want = (z.rows * z.row_bytes + 64 * kZeroThreads - 1) / (64 * kZeroThreads);
+    const int dev = current_device();
+    if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
+    const int64_t most = int64_t(2) * device_info(dev).sm_count;  // leaves the sort room
+    st = launched(launch_dependent(embedding_zero_kernel,
+                                   dim3(static_cast<unsigned>(std::min(want, most))),
+                                   dim3(kZeroThreads), 0, stream, z),
+                  "embedding_zero_kernel");
+    if (st != BEVK_OK) return st;
+    s.behind_zeros = programmatic_launch_enabled();
+  }
+  st = a->ids_are_64bit ? sort_any<int64_t>(s, stream) : sort_any<int32_t>(s, stream);
   if (st != BEVK_OK) return st;
   SumParams p = {};
   p.dy = dy;
   p.out = grad_table;
-  p.key = s.key[(s.passes + 1) & 1];
-  p.pos = s.pos[(s.passes + 1) & 1];
-  p.owners = s.owners;
-  p.owner = s.owner;
+  p.list = s.list[(s.passes + 1) & 1];
+  p.count = s.count;
+  for (int i = 0; i < 2; ++i) p.owner[i] = s.owner[i];
   p.partial = reinterpret_cast<float *>(base + l.partial);
   p.dy_ld = a->grad_output_ld;
   p.out_ld = a->grad_table_ld;

@@ -72,6 +72,18 @@ __device__ __forceinline__ void store_pack(void *p, const Pack<T, VEC> &q) {
     *static_cast<uint16_t *>(p) = static_cast<uint16_t>(q.w[0]);
 }
 
+// The same for data that is not read again soon: it leaves L2 first.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pack_streaming(void *p, const Pack<T, VEC> &q) {
+  using P = Pack<T, VEC>;
+  if constexpr (P::kBytes == 16)
+    __stcs(static_cast<uint4 *>(p), make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]));
+  else if constexpr (P::kBytes == 8)
+    __stcs(static_cast<uint2 *>(p), make_uint2(q.w[0], q.w[1]));
+  else
+    store_pack<T, VEC>(p, q);
+}
+
 __device__ __forceinline__ float2 widen2(uint32_t w, __half) {
   return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
@@ -104,7 +116,7 @@ __device__ __forceinline__ void unpack(const Pack<T, VEC> &q, float (&f)[VEC]) {
   }
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void store(T *p, const float (&f)[VEC]) {
+__device__ __forceinline__ Pack<T, VEC> pack(const float (&f)[VEC]) {
   Pack<T, VEC> q;
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -115,7 +127,11 @@ __device__ __forceinline__ void store(T *p, const float (&f)[VEC]) {
 #pragma unroll
     for (int i = 0; i < VEC / 2; ++i) q.w[i] = narrow2(f[2 * i], f[2 * i + 1], T());
   }
-  store_pack<T, VEC>(p, q);
+  return q;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T *p, const float (&f)[VEC]) {
+  store_pack<T, VEC>(p, pack<T, VEC>(f));
 }
 
 // Two fp32 values in one 64-bit register: Blackwell's packed arithmetic does
