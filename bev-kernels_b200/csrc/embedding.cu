@@ -98,13 +98,8 @@ __device__ __forceinline__ unsigned key_in(Entry e) { return static_cast<unsigne
 
 struct SortParams {
   const void *ids;
-  Entry *list[2];
-  unsigned *hist;     // [cluster size][kDigits]
-  // runs of equal ids that go on past the tile they begin in, as 2 * tile + slot
-  // (slot 1: they begin further in than its first token): of at most kShort
-  // pieces, and of more
-  unsigned *count;    // [2]
-  unsigned *owner[2];
+  Entry *list0, *list1;  // written by the even and the odd passes
+  unsigned *count;       // [2], zeroed for the sums
   int64_t rows, padding;
   int n, passes, cluster;
   int behind_zeros;   // launched while embedding_zero_kernel runs
@@ -163,6 +158,24 @@ __device__ __forceinline__ unsigned warp_scan(unsigned v) {
   return v;
 }
 
+// Lanes (of those in `among`) whose digits equal this one's, by eight votes: the
+// match instruction takes longer the more different values the warp holds.
+__device__ __forceinline__ unsigned equals(unsigned among, unsigned d) {
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const unsigned vote = __ballot_sync(0xffffffffu, (d >> b) & 1u);
+    among &= (d >> b) & 1u ? vote : ~vote;
+  }
+  return among;
+}
+// Reads a word of another CTA's shared memory (of the same cluster).
+__device__ __forceinline__ unsigned load_from_cta(const unsigned *p, int rank) {
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v)
+               : "r"(ptx::mapa_shared(ptx::smem_u32(p), rank)) : "memory");
+  return v;
+}
+
 // Stable least-significant-digit radix sort of (id, position), eight bits a
 // pass.  Every warp owns a stretch of the list.  It counts its digits in order
 // (lanes with equal digits find one another; the first adds them to the warp's
@@ -173,7 +186,9 @@ __device__ __forceinline__ unsigned warp_scan(unsigned v) {
 // them twice.
 template <typename Id, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortParams p) {
+  constexpr int N = ITEMS > 0 ? ITEMS : 1;
   __shared__ alignas(16) unsigned s_cnt[kSortWarps][kDigits];
+  __shared__ unsigned s_total[kDigits];  // of this CTA, read by the cluster
   __shared__ unsigned s_warp[kDigits / 32];
   // behind the zeros everything older is complete already
   if (!p.behind_zeros) ptx::grid_wait_prerequisites();
@@ -185,37 +200,31 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
   const int chunk = ((b1 - b0 + kSortThreads - 1) / kSortThreads) * 32;
   const int w0 = min(b1, b0 + warp * chunk), w1 = min(b1, w0 + chunk);
   const Id *ids = static_cast<const Id *>(p.ids);
-  const auto load = [&](int pass, int i) {
-    return pass ? __ldcg(p.list[(pass + 1) & 1] + i)
-                : entry_of(key_of(ids[i], p), static_cast<unsigned>(i));
-  };
-  // counts a token; returns its rank among the warp's tokens of its digit so far.
-  // Equal digits are found by eight votes: the match instruction takes longer
-  // the more different values the warp holds.
-  const auto tally = [&](bool on, unsigned d) {
-    unsigned same = __ballot_sync(0xffffffffu, on);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const unsigned vote = __ballot_sync(0xffffffffu, (d >> b) & 1u);
-      same &= (d >> b) & 1u ? vote : ~vote;
-    }
-    const unsigned at = on ? s_cnt[warp][d] + __popc(same & ((1u << lane) - 1)) : 0u;
+  const unsigned below = (1u << lane) - 1;
+  // adds the lanes `same` to their digit's counter; returns this lane's rank
+  const auto tally = [&](unsigned same, bool on, unsigned d) {
+    const unsigned at = on ? s_cnt[warp][d] + __popc(same & below) : 0u;
     __syncwarp();
-    if (on && lane == __ffs(same) - 1) s_cnt[warp][d] += __popc(same);
+    if (on && (same & below) == 0) s_cnt[warp][d] += __popc(same);
     __syncwarp();
     return at;
   };
 
   for (int pass = 0; pass < p.passes; ++pass) {
-    Entry *out = p.list[pass & 1];
+    const Entry *in = pass & 1 ? p.list0 : p.list1;
+    Entry *out = pass & 1 ? p.list1 : p.list0;
     const int shift = 32 + 8 * pass;
-    Entry item[ITEMS > 0 ? ITEMS : 1];
-    unsigned at[ITEMS > 0 ? ITEMS : 1];
+    const auto load = [&](int i) {
+      return pass ? __ldcg(in + i) : entry_of(key_of(ids[i], p), static_cast<unsigned>(i));
+    };
+    const auto digit = [&](Entry e) { return static_cast<unsigned>(e >> shift) & (kDigits - 1); };
+    Entry item[N];
+    unsigned at[N];
     if constexpr (ITEMS > 0) {
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
+      for (int k = 0; k < N; ++k) {
         const int i = w0 + k * 32 + lane;
-        item[k] = i < w1 ? load(pass, i) : 0;
+        item[k] = i < w1 ? load(i) : 0;
       }
     }
 #pragma unroll
@@ -224,32 +233,32 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
     __syncthreads();
     if constexpr (ITEMS > 0) {
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k)
-        at[k] = tally(w0 + k * 32 + lane < w1,
-                      static_cast<unsigned>(item[k] >> shift) & (kDigits - 1));
+      for (int k = 0; k < N; ++k)
+        at[k] = equals(__ballot_sync(0xffffffffu, w0 + k * 32 + lane < w1), digit(item[k]));
+#pragma unroll
+      for (int k = 0; k < N; ++k) at[k] = tally(at[k], w0 + k * 32 + lane < w1, digit(item[k]));
     } else {
-      for (int i = w0 + lane; i - lane < w1; i += 32)
-        tally(i < w1, i < w1 ? static_cast<unsigned>(load(pass, i) >> shift) & (kDigits - 1) : 0u);
+      for (int i = w0 + lane; i - lane < w1; i += 32) {
+        const unsigned d = i < w1 ? digit(load(i)) : 0u;
+        tally(equals(__ballot_sync(0xffffffffu, i < w1), d), i < w1, d);
+      }
     }
     __syncthreads();
     // digit totals of the CTA, over the cluster
-    unsigned mine = 0;
     if (tid < kDigits) {
+      unsigned mine = 0;
 #pragma unroll
       for (int w = 0; w < kSortWarps; ++w) mine += s_cnt[w][tid];
-      __stcg(p.hist + rank * kDigits + tid, mine);
+      s_total[tid] = mine;
     }
     ptx::cluster_sync();
     unsigned before = 0, total = 0, scan = 0;
     if (tid < kDigits) {
-      unsigned h[kMostCluster];
-#pragma unroll
-      for (int r = 0; r < kMostCluster; ++r)
-        h[r] = r < p.cluster ? __ldcg(p.hist + r * kDigits + tid) : 0;
 #pragma unroll
       for (int r = 0; r < kMostCluster; ++r) {
-        if (r < rank) before += h[r];
-        total += h[r];
+        const unsigned h = r < p.cluster ? load_from_cta(s_total + tid, r) : 0u;
+        if (r < rank) before += h;
+        total += h;
       }
       scan = warp_scan(total);
       if (lane == 31) s_warp[warp] = scan;
@@ -270,33 +279,18 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
     __syncthreads();
     if constexpr (ITEMS > 0) {
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k)
-        if (w0 + k * 32 + lane < w1)
-          out[s_cnt[warp][static_cast<unsigned>(item[k] >> shift) & (kDigits - 1)] + at[k]] = item[k];
+      for (int k = 0; k < N; ++k)
+        if (w0 + k * 32 + lane < w1) out[s_cnt[warp][digit(item[k])] + at[k]] = item[k];
     } else {
       for (int i = w0 + lane; i - lane < w1; i += 32) {
-        const Entry e = i < w1 ? load(pass, i) : 0;
-        const unsigned to = tally(i < w1, static_cast<unsigned>(e >> shift) & (kDigits - 1));
+        const Entry e = i < w1 ? load(i) : 0;
+        const unsigned to =
+            tally(equals(__ballot_sync(0xffffffffu, i < w1), digit(e)), i < w1, digit(e));
         if (i < w1) out[to] = e;
       }
     }
+    // the next pass reads other CTAs' entries; no CTA leaves while its totals are read
     ptx::cluster_sync();
-  }
-  // runs that go on past the tile they begin in
-  const Entry *list = p.list[(p.passes + 1) & 1];
-  const int tiles = (p.n + kTile - 1) / kTile;
-  for (int t = rank * kSortThreads + tid; t < tiles; t += p.cluster * kSortThreads) {
-    const int64_t first = static_cast<int64_t>(t) * kTile, next = first + kTile;
-    if (next >= p.n) continue;
-    const int64_t far = first + int64_t(kShort) * kTile;  // where a run of more pieces still is
-    const unsigned k = key_in(__ldcg(list + next - 1)), after = key_in(__ldcg(list + next));
-    const unsigned start = key_in(__ldcg(list + first));
-    const unsigned prior = t > 0 ? key_in(__ldcg(list + first - 1)) : ~0u;
-    const unsigned later = far < p.n ? key_in(__ldcg(list + far)) : ~0u;
-    if (k >= static_cast<unsigned>(p.rows) || after != k || prior == k) continue;
-    const int is_long = later == k;
-    // the lists' order changes nothing
-    p.owner[is_long][atomicAdd(p.count + is_long, 1u)] = 2 * t + (start == k ? 0 : 1);
   }
   ptx::grid_launch_dependents();
   if (p.behind_zeros) ptx::grid_wait_prerequisites();
@@ -307,8 +301,11 @@ struct SumParams {
   const void *dy;
   void *out;
   const Entry *list;
-  const unsigned *count;
-  const unsigned *owner[2];
+  // runs of equal ids that go on past the tile they begin in, as 2 * tile + slot
+  // (slot 1: they begin further in than its first token): of at most kShort
+  // pieces, and of more
+  unsigned *count;   // [2]
+  unsigned *owner0, *owner1;
   float *partial;    // [tile][2][pdim]: a run's piece at the tile's start, or further in
   int64_t dy_ld, out_ld;
   int n, rows, dim, pdim, slices;
@@ -358,7 +355,11 @@ __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
 }
 
 constexpr int kSumThreads = 256;
-constexpr int kAhead = 16;  // rows loaded before they are used
+// Rows loaded before they are used.  65536 tokens x 2048 columns of bf16 into
+// fp32 rows take 105 us at 16 rows and 2 CTAs per SM, the same at 8 rows and 2 to
+// 4, 117 at 4 rows and 6; refilling each row's registers as soon as it is
+// summed took 134.
+constexpr int kAhead = 16;
 
 // One warp per (tile, slice of 32 * VEC columns).
 template <typename T, typename O, int VEC>
@@ -407,6 +408,13 @@ __global__ void __launch_bounds__(kSumThreads, 2) embedding_sum_kernel(const Sum
       if ((ends >> t) & 1u) {
         const unsigned row = __shfl_sync(0xffffffffu, key, t);
         const bool open = (begin == 0 && before == row) || (t == kTile - 1 && after == row);
+        if (t == kTile - 1 && after == row && !(begin == 0 && before == row) && c == 0) {
+          // where the run still is if it has more pieces; the lists' order changes nothing
+          const int64_t far = first + int64_t(kShort) * kTile;
+          const bool is_long = far < p.n && key_in(p.list[far]) == row;
+          const unsigned at = atomicAdd(p.count + (is_long ? 1 : 0), 1u);
+          (is_long ? p.owner1 : p.owner0)[at] = static_cast<unsigned>(2 * tile + (begin ? 1 : 0));
+        }
         if (col) {
           if (open) {
             float *dst = p.partial + (tile * 2 + (begin ? 1 : 0)) * p.pdim + c;
@@ -468,7 +476,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumPa
   const int64_t few = static_cast<int64_t>(p.count[0]) * slices;
   const int64_t many = static_cast<int64_t>(p.count[1]) * slices;
   for (int64_t item = blockIdx.x; item < many; item += gridDim.x) {
-    const unsigned o = p.owner[1][item / slices];
+    const unsigned o = p.owner1[item / slices];
     const int c = static_cast<int>(item % slices) * 128 + lane * 4;
     const int64_t tile = o >> 1;
     const unsigned row = key_in(p.list[tile * kTile + kTile - 1]);
@@ -502,7 +510,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumPa
   }
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + warp; item < few;
        item += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const unsigned o = p.owner[0][item / slices];
+    const unsigned o = p.owner0[item / slices];
     const int c = static_cast<int>(item % slices) * 128 + lane * 4;
     const int64_t tile = o >> 1;
     // lane k >= 1: whether the run still is at tile + k; the row from lane 0
@@ -534,7 +542,9 @@ int look(const LookParams &p0, bool wide_ids, cudaStream_t stream) {
   const int64_t want = (p.n + rows - 1) / rows;
   const int dev = current_device();
   if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_forward: no device");
-  const int grid = static_cast<int>(std::min<int64_t>(want, int64_t(64) * device_info(dev).sm_count));
+  // 8 CTAs per SM that loop: 62 us for 65536 rows of 4 KB, against 67 with 64 per SM and
+  // 73 with a CTA for every four rows
+  const int grid = static_cast<int>(std::min<int64_t>(want, int64_t(8) * device_info(dev).sm_count));
   return launched(wide_ids ? launch_dependent(embedding_forward_kernel<T, int64_t, VEC>, dim3(grid),
                                               dim3(kLookThreads), 0, stream, p)
                            : launch_dependent(embedding_forward_kernel<T, int32_t, VEC>, dim3(grid),
@@ -550,7 +560,7 @@ int look_any(const LookParams &p, bool wide_ids, cudaStream_t stream) {
 }
 
 struct Layout {  // of the backward's workspace
-  size_t list[2], hist, count, owner[2], partial, bytes;
+  size_t list[2], count, owner[2], partial, bytes;
   int64_t tiles;
   int pdim;
 };
@@ -569,7 +579,6 @@ Layout layout_of(const bevk_embedding_backward_args *a) {
     l.list[i] = take(n * sizeof(Entry));
     l.owner[i] = take(sizeof(unsigned) * static_cast<size_t>(l.tiles));
   }
-  l.hist = take(sizeof(unsigned) * kMostCluster * kDigits);
   l.count = take(2 * sizeof(unsigned));
   l.partial = take(sizeof(float) * 2 * static_cast<size_t>(l.tiles) * l.pdim);
   l.bytes = at;
@@ -693,11 +702,8 @@ int launch_embedding_backward(const bevk_embedding_backward_args *a, const void 
   char *base = static_cast<char *>(ws);
   SortParams s = {};
   s.ids = ids;
-  for (int i = 0; i < 2; ++i) {
-    s.list[i] = reinterpret_cast<Entry *>(base + l.list[i]);
-    s.owner[i] = reinterpret_cast<unsigned *>(base + l.owner[i]);
-  }
-  s.hist = reinterpret_cast<unsigned *>(base + l.hist);
+  s.list0 = reinterpret_cast<Entry *>(base + l.list[0]);
+  s.list1 = reinterpret_cast<Entry *>(base + l.list[1]);
   s.count = reinterpret_cast<unsigned *>(base + l.count);
   s.rows = a->num_rows;
   s.padding = a->padding_idx;
@@ -725,9 +731,10 @@ int launch_embedding_backward(const bevk_embedding_backward_args *a, const void 
   SumParams p = {};
   p.dy = dy;
   p.out = grad_table;
-  p.list = s.list[(s.passes + 1) & 1];
+  p.list = s.passes & 1 ? s.list0 : s.list1;
   p.count = s.count;
-  for (int i = 0; i < 2; ++i) p.owner[i] = s.owner[i];
+  p.owner0 = reinterpret_cast<unsigned *>(base + l.owner[0]);
+  p.owner1 = reinterpret_cast<unsigned *>(base + l.owner[1]);
   p.partial = reinterpret_cast<float *>(base + l.partial);
   p.dy_ld = a->grad_output_ld;
   p.out_ld = a->grad_table_ld;
