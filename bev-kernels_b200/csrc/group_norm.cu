@@ -41,6 +41,7 @@
 #include <cstdint>
 
 #include "bevk_internal.h"
+#include "bevk_ptx.cuh"
 #include "vec_io.cuh"
 
 namespace cg = cooperative_groups;
@@ -75,6 +76,7 @@ struct GnParams {
   int team, team_log;  // threads that share a group (a power of two)
   int Gb;              // most groups that a channel block touches
   int wave;            // images per wave
+  int cluster;         // 1: an image's CTAs are one thread-block cluster
   int S;               // slabs per image: `longer` of slab + 1 pixels, then of slab
   int slab, longer;
   int keep;            // vectors (backward: pairs) per thread held in shared memory
@@ -374,6 +376,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
   float *s_rstd = s_mean + p.Gb;  // [Gb] each
   cg::grid_group grid = cg::this_grid();
 
+  ptx::grid_launch_dependents();
+  ptx::grid_wait_prerequisites();
   const Place t = place<VEC>(p);
   const int held = min(t.mine, p.keep);
   const int groups = (p.keep + kBatch - 1) / kBatch;  // asynchronous ones, of every thread
@@ -497,8 +501,9 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
     }
     const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
     const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
-    if (p.S > 1 || p.nb > 1) grid.sync();
-    else __syncthreads();
+    if (p.S == 1 && p.nb == 1) __syncthreads();
+    else if (p.cluster) ptx::cluster_sync();
+    else grid.sync();
     const bool next = n + p.wave < p.N;
     if (n < p.N) {
       combine_moments<kThreads>(p, t, n, p.lanes * VEC, s_mean, s_rstd, p.mean != nullptr && t.s == 0);
@@ -865,6 +870,11 @@ void set_lanes(GnParams *p, int vec, int kThreads) {
   p->inv_pitch = 1.f / (p->lanes * vec);
 }
 
+// Pixels per slab at least two for every thread: the most slabs of an image.
+int most_slabs(const GnParams &p) {
+  return static_cast<int>(std::max<int64_t>(1, p.HW / (static_cast<int64_t>(p.R) * 2)));
+}
+
 // Waves and slabs for `ctas` resident CTAs, each with room for `room` vectors
 // of every thread; returns the grid, one CTA per (image of a wave, slab,
 // channel block).  A wave is as many images as the CTAs hold, at least one; the
@@ -875,8 +885,7 @@ int set_slabs(GnParams *p, int ctas, int room) {
       1, std::min<int64_t>(ctas / p->nb, ctas * static_cast<int64_t>(room) / (image * p->nb)));
   const int64_t waves = (p->N + most - 1) / most;
   p->wave = static_cast<int>((p->N + waves - 1) / waves);
-  // a slab holds at least two pixels for every thread
-  const int64_t cut = std::max<int64_t>(1, p->HW / (static_cast<int64_t>(p->R) * 2));
+  const int64_t cut = most_slabs(*p);
   p->S = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(ctas / (static_cast<int64_t>(p->wave) * p->nb), cut)));
   p->slab = p->HW / p->S;
@@ -904,6 +913,61 @@ size_t gpart_bytes(const GnParams &p) {
   return sizeof(float2) * static_cast<size_t>(p.N) * p.nb * p.Gb * p.S;
 }
 
+// Where every image's CTAs can be one cluster, with all clusters resident, they
+// meet at the cluster's barrier instead of the grid's, and the launch is an
+// ordinary one.  That has fewer CTAs than the grid, so it pays while each has
+// little to do: measured against the grid (device time), 64x32x32 f32 6.4 and
+// 7.4 us, 30x128x28x28 bf16 10.6 and 11.6, 6x512x29x50 f16 (12 vectors a thread)
+// 9.8 and 9.9, but 1x256x58x100 bf16 (24 vectors) 15.7 and 9.1.
+// Sets the slabs and returns true where it is used.
+constexpr int kMostHeldByCluster = 12;
+template <auto kernel>
+bool set_clusters(GnParams *p, int room) {
+  if (p->nb > 1) return false;
+  static thread_local int seen_device = -1, fits[17];
+  const int dev = current_device();
+  if (seen_device != dev) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    for (int c : {1, 2, 4, 8, 16}) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = c;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(c);
+      cfg.blockDim = dim3(kForwardThreads);
+      cfg.dynamicSmemBytes = kSmemBytes;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&fits[c], kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        fits[c] = 0;
+      }
+    }
+    seen_device = dev;
+  }
+  const int cut = most_slabs(*p);
+  for (int c : {16, 8, 4, 2, 1}) {
+    if (fits[c] < p->N) continue;
+    const int S = std::min(c, cut);
+    const int slab = (p->HW + S - 1) / S, keep = (slab + p->R - 1) / p->R;
+    if (keep > std::min(room, kMostHeldByCluster)) return false;
+    p->S = S;
+    p->wave = p->N;
+    p->slab = p->HW / S;
+    p->longer = p->HW - p->slab * S;
+    p->slab_rows = p->slab / p->R;
+    p->slab_more = p->slab - p->slab_rows * p->R;
+    p->keep = keep;
+    p->cluster = 1;
+    return true;
+  }
+  return false;
+}
+
 template <auto kernel>
 int launch(GnParams p, int vec, size_t size, bool back, void *ws, size_t ws_bytes,
            cudaStream_t stream) {
@@ -915,7 +979,10 @@ int launch(GnParams p, int vec, size_t size, bool back, void *ws, size_t ws_byte
   p.param_vectors = aligned(p.w, 16) && aligned(p.b, 16);
   const size_t reduce = reduce_bytes(p, vec, back);
   const size_t slot = (back ? 2 : 1) * vec * size;
-  const int grid = set_slabs(&p, ctas, room_for(reduce, slot, threads));
+  const int room = room_for(reduce, slot, threads);
+  int grid = set_slabs(&p, ctas, room);
+  const bool clusters = !back && set_clusters<kernel>(&p, room);
+  if (clusters) grid = p.N * p.S;
   const size_t cpart = back ? static_cast<size_t>(grid) * p.lanes * vec : 0;
   const size_t need = cpart * sizeof(float2) + gpart_bytes(p);
   if (ws_bytes < need)
@@ -923,6 +990,22 @@ int launch(GnParams p, int vec, size_t size, bool back, void *ws, size_t ws_byte
                 need);
   p.cpart = static_cast<float2 *>(ws);
   p.gpart = p.cpart + cpart;
+  if (clusters) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = reduce + p.keep * slot * threads;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = programmatic_launch_enabled() ? 2 : 1;
+    return launched(cudaLaunchKernelEx(&cfg, kernel, p), "gn_forward_kernel");
+  }
   void *args[] = {&p};
   return launched(cudaLaunchCooperativeKernel(reinterpret_cast<void *>(kernel), dim3(grid),
                                               dim3(threads), args, reduce + p.keep * slot * threads,
@@ -1004,7 +1087,7 @@ size_t group_norm_workspace_bytes(const bevk_group_norm_problem *q, bool backwar
     if (q->channels % vec) continue;
     GnParams p = base_params(q);
     set_lanes(&p, vec, threads_of(backward));
-    const int64_t cut = std::max<int64_t>(1, p.HW / (static_cast<int64_t>(p.R) * 2));
+    const int64_t cut = most_slabs(p);
     p.S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostCtas / p.nb, cut)));
     size_t n = gpart_bytes(p);
     if (backward) n += sizeof(float2) * kMostCtas * static_cast<size_t>(p.lanes) * vec;
