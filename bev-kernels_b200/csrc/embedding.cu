@@ -355,15 +355,20 @@ __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
 }
 
 constexpr int kSumThreads = 256;
-// Rows loaded before they are used.  65536 tokens x 2048 columns of bf16 into
-// fp32 rows take 105 us at 16 rows and 2 CTAs per SM, the same at 8 rows and 2 to
-// 4, 117 at 4 rows and 6; refilling each row's registers as soon as it is
-// summed took 134.
+// Rows on their way per warp.  Where a thread's part of a row is 16 bytes they
+// are copied asynchronously into slots of its own in shared memory; the loop
+// over the tile's tokens then stays short, and a warp waits for its next row
+// only.  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with 16
+// rows and 3 CTAs per SM, 104 to 108 with 4 to 24 rows and 8 to 2, and with
+// batches of 16 rows in registers.
 constexpr int kAhead = 16;
 
 // One warp per (tile, slice of 32 * VEC columns).
 template <typename T, typename O, int VEC>
-__global__ void __launch_bounds__(kSumThreads, 2) embedding_sum_kernel(const SumParams p) {
+__global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const SumParams p) {
+  constexpr bool kAsync = sizeof(T) * VEC == 16;
+  constexpr int kSlot = 32 * 16;
+  extern __shared__ float4 s_dyn[];  // [warp][kAhead][lane] where copies are asynchronous
   ptx::grid_launch_dependents();
   ptx::grid_wait_prerequisites();
   const int lane = threadIdx.x & 31;
@@ -383,59 +388,70 @@ __global__ void __launch_bounds__(kSumThreads, 2) embedding_sum_kernel(const Sum
   const unsigned ends = __ballot_sync(0xffffffffu, lane == 31 || key != next);
   const T *dy = static_cast<const T *>(p.dy) + c;
   const bool col = c < p.dim;
+  char *ring = reinterpret_cast<char *>(s_dyn) + (threadIdx.x >> 5) * kAhead * kSlot + lane * 16;
+  const auto row_of = [&](int t) {  // token t's row of dy, for the whole warp
+    return dy + static_cast<int64_t>(__shfl_sync(0xffffffffu, pos, t & 31)) * p.dy_ld;
+  };
+  const auto fetch = [&](int t) {
+    const T *src = row_of(t);
+    if (col && t < count) vio::copy_async16(ring + t % kAhead * kSlot, src);
+    vio::copy_commit();
+  };
+  if constexpr (kAsync) {
+#pragma unroll 4
+    for (int t = 0; t < kAhead; ++t) fetch(t);
+  }
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   int begin = 0;
-  for (int j0 = 0; j0 < count; j0 += kAhead) {
-    vio::Pack<T, VEC> q[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const unsigned at = __shfl_sync(0xffffffffu, pos, (j0 + j) & 31);
-      if (col && j0 + j < count)
-        q[j] = vio::load_pack<T, VEC>(dy + static_cast<int64_t>(at) * p.dy_ld);
+#pragma unroll 1
+  for (int t = 0; t < count; ++t) {
+    vio::Pack<T, VEC> q;
+    if constexpr (kAsync) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      q = vio::load_pack<T, VEC>(ring + t % kAhead * kSlot);
+    } else {
+      const T *src = row_of(t);
+      if (col) q = vio::load_pack<T, VEC>(src);
     }
+    if (col) {
+      float v[VEC];
+      vio::unpack(q, v);
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int t = j0 + j;
-      if (t >= count) break;
-      if (col) {
-        float v[VEC];
-        vio::unpack(q[j], v);
+      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    }
+    if constexpr (kAsync) fetch(t + kAhead);
+    if (!((ends >> t) & 1u)) continue;
+    const unsigned row = __shfl_sync(0xffffffffu, key, t);
+    const bool goes_on = t == kTile - 1 && after == row;
+    const bool open = (begin == 0 && before == row) || goes_on;
+    if (goes_on && !(begin == 0 && before == row) && c == 0) {
+      // where the run still is if it has more pieces; the lists' order changes nothing
+      const int64_t far = first + int64_t(kShort) * kTile;
+      const bool is_long = far < p.n && key_in(p.list[far]) == row;
+      const unsigned at = atomicAdd(p.count + (is_long ? 1 : 0), 1u);
+      (is_long ? p.owner1 : p.owner0)[at] = static_cast<unsigned>(2 * tile + (begin ? 1 : 0));
+    }
+    if (col) {
+      if (open) {
+        float *dst = p.partial + (tile * 2 + (begin ? 1 : 0)) * p.pdim + c;
+        if constexpr (VEC % 4 == 0) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
-      }
-      if ((ends >> t) & 1u) {
-        const unsigned row = __shfl_sync(0xffffffffu, key, t);
-        const bool open = (begin == 0 && before == row) || (t == kTile - 1 && after == row);
-        if (t == kTile - 1 && after == row && !(begin == 0 && before == row) && c == 0) {
-          // where the run still is if it has more pieces; the lists' order changes nothing
-          const int64_t far = first + int64_t(kShort) * kTile;
-          const bool is_long = far < p.n && key_in(p.list[far]) == row;
-          const unsigned at = atomicAdd(p.count + (is_long ? 1 : 0), 1u);
-          (is_long ? p.owner1 : p.owner0)[at] = static_cast<unsigned>(2 * tile + (begin ? 1 : 0));
+          for (int k = 0; k < VEC; k += 4)
+            __stcg(reinterpret_cast<float4 *>(dst + k),
+                   make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) __stcg(dst + k, acc[k]);
         }
-        if (col) {
-          if (open) {
-            float *dst = p.partial + (tile * 2 + (begin ? 1 : 0)) * p.pdim + c;
-            if constexpr (VEC % 4 == 0) {
-#pragma unroll
-              for (int k = 0; k < VEC; k += 4)
-                __stcg(reinterpret_cast<float4 *>(dst + k),
-                       make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]));
-            } else {
-#pragma unroll
-              for (int k = 0; k < VEC; ++k) __stcg(dst + k, acc[k]);
-            }
-          } else {
-            finish<O, VEC>(p, row, c, acc);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-        begin = t + 1;
+      } else {
+        finish<O, VEC>(p, row, c, acc);
       }
     }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    begin = t + 1;
   }
 }
 
@@ -655,9 +671,22 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
   const int64_t grid = (warps + per - 1) / per;
   if (grid >= (int64_t(1) << 31))
     return fail(BEVK_ERR_INDEX_OVERFLOW, "embedding_backward: too many tokens and columns");
+  const size_t smem = sizeof(T) * VEC == 16 ? size_t(16) * kAhead * kSumThreads : 0;
+  if (smem > 0) {
+    static thread_local int seen_device = -1;
+    const int dev = current_device();
+    if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
+    if (seen_device != dev) {
+      const cudaError_t e = cudaFuncSetAttribute(embedding_sum_kernel<T, O, VEC>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(smem));
+      if (e != cudaSuccess) return launched(e, "embedding_sum_kernel");
+      seen_device = dev;
+    }
+  }
   const int st = launched(launch_dependent(embedding_sum_kernel<T, O, VEC>,
-                                           dim3(static_cast<unsigned>(grid)), dim3(kSumThreads), 0,
-                                           stream, p),
+                                           dim3(static_cast<unsigned>(grid)), dim3(kSumThreads),
+                                           smem, stream, p),
                           "embedding_sum_kernel");
   if (st != BEVK_OK) return st;
   if (tiles < 2) return BEVK_OK;  // no run crosses tiles
