@@ -355,10 +355,10 @@ __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
 }
 
 constexpr int kSumThreads = 256;
-// Rows on their way per warp.  Where a thread's part of a row is 16 bytes they
-// are copied asynchronously into slots of its own in shared memory; the loop
-// over the tile's tokens then stays short, and a warp waits for its next row
-// only.  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with 16
+// Rows on their way per warp: every thread copies its part of them asynchronously
+// into slots of its own in shared memory, so the loop over the tile's tokens is
+// short and a warp waits for its next row only.  (Parts of two bytes, which
+// cannot be copied so, are loaded kAhead at a time instead.)  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with 16
 // rows and 3 CTAs per SM, 104 to 108 with 4 to 24 rows and 8 to 2, and with
 // batches of 16 rows in registers.
 constexpr int kAhead = 16;
@@ -366,8 +366,9 @@ constexpr int kAhead = 16;
 // One warp per (tile, slice of 32 * VEC columns).
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const SumParams p) {
-  constexpr bool kAsync = sizeof(T) * VEC == 16;
-  constexpr int kSlot = 32 * 16;
+  constexpr int kBytes = sizeof(T) * VEC;
+  constexpr bool kAsync = kBytes >= 4;
+  constexpr int kSlot = 32 * kBytes;
   extern __shared__ float4 s_dyn[];  // [warp][kAhead][lane] where copies are asynchronous
   ptx::grid_launch_dependents();
   ptx::grid_wait_prerequisites();
@@ -388,13 +389,13 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
   const unsigned ends = __ballot_sync(0xffffffffu, lane == 31 || key != next);
   const T *dy = static_cast<const T *>(p.dy) + c;
   const bool col = c < p.dim;
-  char *ring = reinterpret_cast<char *>(s_dyn) + (threadIdx.x >> 5) * kAhead * kSlot + lane * 16;
+  char *ring = reinterpret_cast<char *>(s_dyn) + (threadIdx.x >> 5) * kAhead * kSlot + lane * kBytes;
   const auto row_of = [&](int t) {  // token t's row of dy, for the whole warp
     return dy + static_cast<int64_t>(__shfl_sync(0xffffffffu, pos, t & 31)) * p.dy_ld;
   };
   const auto fetch = [&](int t) {
     const T *src = row_of(t);
-    if (col && t < count) vio::copy_async16(ring + t % kAhead * kSlot, src);
+    if (col && t < count) vio::copy_async<kAsync ? kBytes : 4>(ring + t % kAhead * kSlot, src);
     vio::copy_commit();
   };
   if constexpr (kAsync) {
@@ -405,15 +406,24 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   int begin = 0;
+  vio::Pack<T, VEC> batch[kAsync ? 1 : kAhead];
 #pragma unroll 1
   for (int t = 0; t < count; ++t) {
     vio::Pack<T, VEC> q;
-    if constexpr (kAsync) {
+    if constexpr (!kAsync) {
+      if (t % kAhead == 0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const T *src = row_of(t + j);
+          if (col && t + j < count) batch[j] = vio::load_pack<T, VEC>(src);
+        }
+      }
+      q = batch[0];
+#pragma unroll
+      for (int j = 0; j + 1 < kAhead; ++j) batch[j] = batch[j + 1];
+    } else {
       asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
       q = vio::load_pack<T, VEC>(ring + t % kAhead * kSlot);
-    } else {
-      const T *src = row_of(t);
-      if (col) q = vio::load_pack<T, VEC>(src);
     }
     if (col) {
       float v[VEC];
@@ -568,11 +578,14 @@ int look(const LookParams &p0, bool wide_ids, cudaStream_t stream) {
                   "embedding_forward_kernel");
 }
 
-template <typename T>
+template <typename T, int VEC = vio::Full<T>::value>
 int look_any(const LookParams &p, bool wide_ids, cudaStream_t stream) {
-  constexpr int V = vio::Full<T>::value;
-  const bool vectors = p.dim % V == 0 && p.ld % V == 0 && aligned(p.table, 16) && aligned(p.out, 16);
-  return vectors ? look<T, V>(p, wide_ids, stream) : look<T, 1>(p, wide_ids, stream);
+  const bool fits = p.dim % VEC == 0 && p.ld % VEC == 0 && aligned(p.table, VEC * sizeof(T)) &&
+                    aligned(p.out, VEC * sizeof(T));
+  if constexpr (VEC > 1) {
+    if (!fits) return look_any<T, VEC / 2>(p, wide_ids, stream);
+  }
+  return look<T, VEC>(p, wide_ids, stream);
 }
 
 struct Layout {  // of the backward's workspace
@@ -601,66 +614,79 @@ Layout layout_of(const bevk_embedding_backward_args *a) {
   return l;
 }
 
-// CTAs of the sorting cluster: a token a thread, up to the hardware's most (16
-// where a cluster of that size fits on the device, else 8).
-int cluster_size(int64_t n) {
-  int c = 1;
-  while (c < kMostCluster && n > int64_t(kSortThreads) * c) c <<= 1;
-  return c;
-}
-
-template <auto kernel>
-int sort_ids(const SortParams &p0, int cluster, cudaStream_t stream) {
-  SortParams p = p0;
-  const int dev = current_device();
-  if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
-  p.cluster = cluster;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
+template <typename Id, int ITEMS>
+void sort_config(cudaLaunchConfig_t *cfg, cudaLaunchAttribute (&attr)[2], int cluster) {
+  *cfg = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = programmatic_launch_enabled() ? 2 : 1;
-  cfg.gridDim = dim3(p.cluster);
-  if (p.cluster > 8) {
-    static thread_local int seen_device = -1, fits = 0;
+  cfg->gridDim = dim3(cluster);
+  cfg->blockDim = dim3(kSortThreads);
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+}
+
+template <typename Id, int ITEMS>
+int sort_ids(SortParams p, int cluster, cudaStream_t stream) {
+  auto kernel = embedding_sort_kernel<Id, ITEMS>;
+  p.cluster = cluster;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  sort_config<Id, ITEMS>(&cfg, attr, cluster);
+  if (cluster > 8) {
+    static thread_local int seen_device = -1;
+    const int dev = current_device();
     if (seen_device != dev) {
-      const unsigned attrs = cfg.numAttrs;
-      cfg.numAttrs = 1;
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
-              cudaSuccess ||
-          cudaOccupancyMaxActiveClusters(&fits, kernel, &cfg) != cudaSuccess) {
-        (void)cudaGetLastError();
-        fits = 0;
-      }
-      cfg.numAttrs = attrs;
+      const cudaError_t e =
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return launched(e, "embedding_sort_kernel");
       seen_device = dev;
     }
-    if (fits < 1) attr[0].val.clusterDim.x = p.cluster = 8;
   }
-  cfg.gridDim = dim3(p.cluster);
+  cfg.stream = stream;
+  cfg.numAttrs = programmatic_launch_enabled() ? 2 : 1;
   return launched(cudaLaunchKernelEx(&cfg, kernel, p), "embedding_sort_kernel");
 }
 
-// Picks the tokens that a thread keeps in registers.
+// The largest sorting cluster of the current device: 16 CTAs where one of that
+// size fits, else the 8 that every device takes (0 on an error).
+int most_sorting_ctas() {
+  static thread_local int seen_device = -1, most = 8;
+  const int dev = current_device();
+  if (dev < 0) return 0;
+  if (seen_device == dev) return most;
+  auto kernel = embedding_sort_kernel<int64_t, 8>;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  sort_config<int64_t, 8>(&cfg, attr, kMostCluster);
+  int fits = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+          cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&fits, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    fits = 0;
+  }
+  most = fits > 0 ? kMostCluster : 8;
+  seen_device = dev;
+  return most;
+}
+
+// A token a thread up to the largest cluster, then 2, 4 or 8 a thread in
+// registers, then any number.
 template <typename Id>
 int sort_any(const SortParams &p, cudaStream_t stream) {
-  const int cluster = cluster_size(p.n);
-  // the half-sized cluster of a device without room for 16 CTAs holds twice as many each
-  const int64_t each = (p.n + cluster - 1) / cluster * (cluster > 8 ? 2 : 1);
-  if (each <= kSortThreads) return sort_ids<embedding_sort_kernel<Id, 1>>(p, cluster, stream);
-  if (each <= 2 * kSortThreads)
-    return sort_ids<embedding_sort_kernel<Id, 2>>(p, cluster, stream);
-  if (each <= 4 * kSortThreads)
-    return sort_ids<embedding_sort_kernel<Id, 4>>(p, cluster, stream);
-  if (each <= 8 * kSortThreads)
-    return sort_ids<embedding_sort_kernel<Id, 8>>(p, cluster, stream);
-  return sort_ids<embedding_sort_kernel<Id, 0>>(p, cluster, stream);
+  const int most = most_sorting_ctas();
+  if (most == 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
+  int cluster = 1;
+  while (cluster < most && p.n > kSortThreads * cluster) cluster *= 2;
+  const int each = (p.n + cluster - 1) / cluster;
+  if (each <= kSortThreads) return sort_ids<Id, 1>(p, cluster, stream);
+  if (each <= 2 * kSortThreads) return sort_ids<Id, 2>(p, cluster, stream);
+  if (each <= 4 * kSortThreads) return sort_ids<Id, 4>(p, cluster, stream);
+  if (each <= 8 * kSortThreads) return sort_ids<Id, 8>(p, cluster, stream);
+  return sort_ids<Id, 0>(p, cluster, stream);
 }
 
 template <typename T, typename O, int VEC>
@@ -671,7 +697,7 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
   const int64_t grid = (warps + per - 1) / per;
   if (grid >= (int64_t(1) << 31))
     return fail(BEVK_ERR_INDEX_OVERFLOW, "embedding_backward: too many tokens and columns");
-  const size_t smem = sizeof(T) * VEC == 16 ? size_t(16) * kAhead * kSumThreads : 0;
+  const size_t smem = sizeof(T) * VEC >= 4 ? sizeof(T) * VEC * kAhead * kSumThreads : 0;
   if (smem > 0) {
     static thread_local int seen_device = -1;
     const int dev = current_device();
@@ -699,13 +725,17 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
                   "embedding_join_kernel");
 }
 
-template <typename T, typename O>
+// The widest part of a row, up to 16 bytes, that every row's start and length are
+// a multiple of on the side of dy, and its columns on the side of the table.
+template <typename T, typename O, int VEC = vio::Full<T>::value>
 int sum_any(const SumParams &p, int64_t tiles, cudaStream_t stream) {
-  constexpr int V = vio::Full<T>::value;
-  const bool vectors = p.dim % V == 0 && p.dy_ld % V == 0 &&
-                       p.out_ld * sizeof(O) % 16 == 0 &&
-                       aligned(p.dy, 16) && aligned(p.out, 16);
-  return vectors ? sum<T, O, V>(p, tiles, stream) : sum<T, O, 1>(p, tiles, stream);
+  constexpr size_t kOut = std::min<size_t>(16, VEC * sizeof(O));
+  const bool fits = p.dim % VEC == 0 && p.dy_ld % VEC == 0 && aligned(p.dy, VEC * sizeof(T)) &&
+                    p.out_ld * sizeof(O) % kOut == 0 && aligned(p.out, kOut);
+  if constexpr (VEC > 1) {
+    if (!fits) return sum_any<T, O, VEC / 2>(p, tiles, stream);
+  }
+  return sum<T, O, VEC>(p, tiles, stream);
 }
 
 }  // namespace

@@ -38,7 +38,8 @@ constexpr int kCtasPerSm = 2;
 constexpr int kBatch = 4;
 constexpr int kMostTile = 32768;  // elements
 constexpr int kMostTensors = 1000;  // of one launch: 32 KB of kernel parameters hold them
-constexpr int kFewTensors = 100;    // fit the first 4 KB of parameters
+constexpr int kSomeTensors = 400;   // parameters are copied at every launch, so there are
+constexpr int kFewTensors = 100;    // kernels for 12 KB and 3 KB of them too
 constexpr int kMostCtas = 148 * 4;
 
 enum Mode { kBoth = 0, kNormOnly = 1, kScaleOnly = 2 };
@@ -331,33 +332,39 @@ int launch(const bevk_grad_tensor *tensors, int n, const Call &c, Mode mode, int
 int chunks_of(int tensors) { return std::max(1, (tensors + kMostTensors - 1) / kMostTensors); }
 
 // Outputs are disjoint from one another and from every gradient but their own.
+// Two lists, since tensors of one buffer mostly come in order and then nothing
+// has to be sorted.
 int check_overlap(const bevk_grad_tensor *t, int n) {
   struct Span {
     uintptr_t begin, end;
     int tensor;
-    bool out;
   };
-  std::vector<Span> spans;
-  spans.reserve(2 * static_cast<size_t>(n));
-  bool sorted = true;
+  std::vector<Span> outs, grads;  // a gradient scaled in place is an output only
+  outs.reserve(static_cast<size_t>(n));
+  grads.reserve(static_cast<size_t>(n));
   for (int i = 0; i < n; ++i) {
     if (t[i].numel == 0) continue;
     const auto a = reinterpret_cast<uintptr_t>(t[i].out);
     const auto b = reinterpret_cast<uintptr_t>(t[i].grad);
-    spans.push_back({a, a + t[i].numel * dtype_size(t[i].out_dtype), i, true});
+    outs.push_back({a, a + t[i].numel * dtype_size(t[i].out_dtype), i});
     if (t[i].grad != t[i].out)
-      spans.push_back({b, b + t[i].numel * dtype_size(t[i].grad_dtype), i, false});
+      grads.push_back({b, b + t[i].numel * dtype_size(t[i].grad_dtype), i});
   }
   const auto less = [](const Span &x, const Span &y) { return x.begin < y.begin; };
-  sorted = std::is_sorted(spans.begin(), spans.end(), less);
-  if (!sorted) std::sort(spans.begin(), spans.end(), less);
-  uintptr_t out_end = 0, any_end = 0;
-  for (const Span &s : spans) {
-    if (s.begin < out_end || (s.out && s.begin < any_end))
+  for (std::vector<Span> *v : {&outs, &grads})
+    if (!std::is_sorted(v->begin(), v->end(), less)) std::sort(v->begin(), v->end(), less);
+  // in order of address over both: no output before the end of anything, no
+  // gradient before the end of an output
+  uintptr_t out_end = 0, grad_end = 0;
+  size_t i = 0, j = 0;
+  while (i < outs.size() || j < grads.size()) {
+    const bool out = j == grads.size() || (i < outs.size() && outs[i].begin <= grads[j].begin);
+    const Span &s = out ? outs[i++] : grads[j++];
+    if (s.begin < out_end || (out && s.begin < grad_end))
       return fail(BEVK_ERR_INVALID_ARGUMENT,
                   "grad_clip: tensor %d overlaps another tensor that is written or read", s.tensor);
-    any_end = std::max(any_end, s.end);
-    if (s.out) out_end = std::max(out_end, s.end);
+    uintptr_t &end = out ? out_end : grad_end;
+    end = std::max(end, s.end);
   }
   return BEVK_OK;
 }
@@ -382,6 +389,7 @@ int launch_grad_clip(const bevk_grad_tensor *tensors, int n, int norm_kind, floa
                   static_cast<double *>(ws)};
   int partials = 0;
   if (n <= kFewTensors) return launch<kFewTensors>(tensors, n, c, kBoth, &partials, true, stream);
+  if (n <= kSomeTensors) return launch<kSomeTensors>(tensors, n, c, kBoth, &partials, true, stream);
   if (n <= kMostTensors) return launch<kMostTensors>(tensors, n, c, kBoth, &partials, true, stream);
   // more tensors than one launch's parameters hold: the norms first, then the
   // scaling, a launch per 1000 tensors each

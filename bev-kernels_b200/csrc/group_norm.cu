@@ -353,7 +353,7 @@ constexpr bool kAsync = sizeof(T) * VEC == 16;
 
 template <typename T, int VEC>
 __device__ __forceinline__ void fetch(char *slot, const T *src) {
-  if constexpr (kAsync<T, VEC>) vio::copy_async16(slot, src);
+  if constexpr (kAsync<T, VEC>) vio::copy_async<16>(slot, src);
   else vio::store_pack<T, VEC>(slot, vio::load_pack<T, VEC>(src));
 }
 

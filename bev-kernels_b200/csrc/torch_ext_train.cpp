@@ -278,12 +278,26 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
                                                            : std::nullopt);
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor &g = grads[i];
-    check_cuda(g, "gradient");
-    check_same_device(first, g, "gradient");
+    if (g.device() != first.device() || !g.is_cuda()) {
+      check_cuda(g, "gradient");
+      check_same_device(first, g, "gradient");
+    }
     TORCH_CHECK(g.layout() == at::kStrided, "bevk: gradients must be strided tensors");
     bevk_grad_tensor &it = items[i];
     it.grad_dtype = dtype_of(g);
     it.numel = g.numel();
+    if (g.is_contiguous() && (!max_norm || !out)) {  // the common cases, without copies
+      it.grad = it.out = g.data_ptr();
+      it.out_dtype = it.grad_dtype;
+      continue;
+    }
+    if (g.is_contiguous() && (*out)[i].is_contiguous() && (*out)[i].sizes() == g.sizes() &&
+        (*out)[i].device() == g.device()) {
+      it.grad = g.data_ptr();
+      it.out = (*out)[i].data_ptr();
+      it.out_dtype = dtype_of((*out)[i]);
+      continue;
+    }
     Tensor src = g;
     if (!max_norm) {
       if (!dense(src)) keep.push_back(src = src.contiguous());

@@ -272,13 +272,17 @@ __device__ __forceinline__ void params_to_float(const Params<VEC> &q, const void
   }
 }
 
-// Asynchronous 16-byte copies from global to shared memory, in groups that
-// complete in order.
-__device__ __forceinline__ void copy_async16(void *smem, const void *global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
-               "l"(global)
-               : "memory");
+// Asynchronous copies of 4, 8 or 16 bytes from global to shared memory, in
+// groups that complete in order.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void *smem, const void *global) {
+  static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16, "one copy");
+  const auto to = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(BYTES)
+                 : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `pending` (0 to 7) of the thread's groups are not complete.
