@@ -38,8 +38,7 @@ constexpr int kCtasPerSm = 2;
 constexpr int kBatch = 4;
 constexpr int kMostTile = 32768;  // elements
 constexpr int kMostTensors = 1000;  // of one launch: 32 KB of kernel parameters hold them
-constexpr int kSomeTensors = 400;   // parameters are copied at every launch, so there are
-constexpr int kFewTensors = 100;    // kernels for 12 KB and 3 KB of them too
+constexpr int kFewTensors = 100;    // fit the first 4 KB of parameters
 constexpr int kMostCtas = 148 * 4;
 
 enum Mode { kBoth = 0, kNormOnly = 1, kScaleOnly = 2 };
@@ -389,7 +388,6 @@ int launch_grad_clip(const bevk_grad_tensor *tensors, int n, int norm_kind, floa
                   static_cast<double *>(ws)};
   int partials = 0;
   if (n <= kFewTensors) return launch<kFewTensors>(tensors, n, c, kBoth, &partials, true, stream);
-  if (n <= kSomeTensors) return launch<kSomeTensors>(tensors, n, c, kBoth, &partials, true, stream);
   if (n <= kMostTensors) return launch<kMostTensors>(tensors, n, c, kBoth, &partials, true, stream);
   // more tensors than one launch's parameters hold: the norms first, then the
   // scaling, a launch per 1000 tensors each

@@ -1,6 +1,8 @@
 // torch_ext_train.cpp -- module _bevk_train_ext: the training-side operators
 // (group norm with activation on channels-last tensors, embedding lookup with
 // scaling, the global gradient norm and clipping) over the C ABI.
+#include <c10/cuda/CUDACachingAllocator.h>
+
 #include <optional>
 #include <string>
 #include <tuple>
@@ -103,8 +105,10 @@ bevk_group_norm_problem gn_problem(const Tensor &input, int64_t num_groups,
   return p;
 }
 
-Tensor scratch(size_t bytes, const Tensor &like) {
-  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+// Scratch memory of the current device and stream, back to torch's allocator at
+// the end of the scope (and half the host time of a tensor).
+c10::DataPtr scratch(size_t bytes) {
+  return c10::cuda::CUDACachingAllocator::get()->allocate(std::max<size_t>(bytes, 1));
 }
 
 std::tuple<Tensor, OptTensor, OptTensor> group_norm_act_forward(
@@ -123,11 +127,11 @@ std::tuple<Tensor, OptTensor, OptTensor> group_norm_act_forward(
     rstd = at::empty({input.size(0), num_groups}, opt);
   }
   const size_t bytes = bevk_group_norm_act_workspace_bytes(&p, 0);
-  const Tensor ws = scratch(bytes, input);
+  const c10::DataPtr ws = scratch(bytes);
   check_status(bevk_group_norm_act_forward(
                    &p, input.data_ptr(), ptr(weight), ptr(bias), output.data_ptr(),
                    stats ? mean->data_ptr<float>() : nullptr,
-                   stats ? rstd->data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
+                   stats ? rstd->data_ptr<float>() : nullptr, ws.get(), bytes,
                    current_stream(input)),
                "group_norm_act_forward");
   return {output, mean, rstd};
@@ -160,12 +164,12 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(
   if (need_weight) gw = at::empty({input.size(1)}, popt);
   if (need_bias) gb = at::empty({input.size(1)}, popt);
   const size_t bytes = bevk_group_norm_act_workspace_bytes(&p, 1);
-  const Tensor ws = scratch(bytes, input);
+  const c10::DataPtr ws = scratch(bytes);
   const auto out = [](const OptTensor &t) { return t ? t->data_ptr() : nullptr; };
   check_status(bevk_group_norm_act_backward(
                    &p, grad_output.data_ptr(), input.data_ptr(), mean.data_ptr<float>(),
                    rstd.data_ptr<float>(), ptr(weight), ptr(bias), out(gi), out(gw), out(gb),
-                   ws.data_ptr(), bytes, current_stream(input)),
+                   ws.get(), bytes, current_stream(input)),
                "group_norm_act_backward");
   return {gi, gw, gb};
 }
@@ -246,9 +250,9 @@ Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t
   a.scale = static_cast<float>(scale);
   a.accumulate = into.has_value();
   const size_t bytes = bevk_embedding_backward_workspace_bytes(&a);
-  const Tensor ws = scratch(bytes, grad_output);
+  const c10::DataPtr ws = scratch(bytes);
   check_status(bevk_embedding_backward(&a, dy.data_ptr(), ids.data_ptr(), out.data_ptr(),
-                                       ws.data_ptr(), bytes, current_stream(grad_output)),
+                                       ws.get(), bytes, current_stream(grad_output)),
                "embedding_backward");
   return out;
 }
@@ -336,11 +340,11 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
   }
   Tensor norm = at::empty({}, first.options().dtype(at::kFloat));
   const size_t bytes = bevk_grad_clip_workspace_bytes(static_cast<int>(items.size()));
-  const Tensor ws = scratch(bytes, first);
+  const c10::DataPtr ws = scratch(bytes);
   check_status(bevk_grad_clip(items.data(), static_cast<int>(items.size()),
                               inf_norm ? BEVK_NORM_INF : BEVK_NORM_L2,
                               static_cast<float>(max_norm.value_or(0.0)), static_cast<float>(eps),
-                              max_norm.has_value(), norm.data_ptr<float>(), ws.data_ptr(), bytes,
+                              max_norm.has_value(), norm.data_ptr<float>(), ws.get(), bytes,
                               current_stream(first)),
                "grad_clip");
   for (auto &c : copy_back) c.first.copy_(c.second);

@@ -90,8 +90,9 @@ def group_norm_act(input: torch.Tensor, num_groups: int, weight: torch.Tensor | 
                    bias: torch.Tensor | None = None, eps: float = 1e-5,
                    act: str = "none") -> torch.Tensor:
     """Group norm and activation; differentiable in input, weight and bias."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (input, weight, bias)):
+    if torch.is_grad_enabled() and (input.requires_grad
+                                    or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return GroupNormActFunction.apply(input, num_groups, weight, bias, eps, act)
     return _load_ext().group_norm_act_forward(input, num_groups, weight, bias, eps, _act(act),
                                               False)[0]
