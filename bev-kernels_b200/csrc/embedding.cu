@@ -15,9 +15,18 @@
 // same work whatever the ids are -- and walks it in order with fp32 sums in
 // registers.  A run of equal ids that lies inside its tile is finished there;
 // the pieces of a run that crosses tiles go to scratch and a last kernel adds
-// them in order.  The sort runs on one thread-block cluster (its passes meet
-// at the cluster's hardware barrier, keys and positions stay in L2) while the
-// other SMs write the zeros of a dense gradient, which are most of its bytes.
+// them in order.  The sort runs on one thread-block cluster: its passes meet
+// at the cluster's hardware barrier and exchange their digit totals through
+// distributed shared memory, the list stays in L2.  The zeros of a dense
+// gradient, most of its bytes, are written by another kernel at the same time.
+//
+// Bound by memory at many tokens (writes alone reach 3.7 to 4 TB/s on this part,
+// reads 5 at these sizes), by the chain of launches and the sort at few.
+// Device time: 65536 rows of 4 KB looked up in 61 us (333 MB, 5.4 TB/s); their
+// gradient added to 10000 fp32 rows in 136 us (430 MB; the sort 20 us of it);
+// 16384 tokens into a dense 50021 x 1024 bf16 table in 41 us (136 MB); 40000
+// tokens of 200 rows of 512 bytes in 19 us, of which the sort is 9; 30 tokens in
+// 12 us, the launches of zeros, sort and sums.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -201,6 +210,11 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
   const int w0 = min(b1, b0 + warp * chunk), w1 = min(b1, w0 + chunk);
   const Id *ids = static_cast<const Id *>(p.ids);
   const unsigned below = (1u << lane) - 1;
+  // a cluster of one CTA spares itself the wider barrier's fence
+  const auto meet = [&] {
+    if (p.cluster == 1) __syncthreads();
+    else ptx::cluster_sync();
+  };
   // adds the lanes `same` to their digit's counter; returns this lane's rank
   const auto tally = [&](unsigned same, bool on, unsigned d) {
     const unsigned at = on ? s_cnt[warp][d] + __popc(same & below) : 0u;
@@ -251,7 +265,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
       for (int w = 0; w < kSortWarps; ++w) mine += s_cnt[w][tid];
       s_total[tid] = mine;
     }
-    ptx::cluster_sync();
+    meet();
     unsigned before = 0, total = 0, scan = 0;
     if (tid < kDigits) {
 #pragma unroll
@@ -290,7 +304,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
       }
     }
     // the next pass reads other CTAs' entries; no CTA leaves while its totals are read
-    ptx::cluster_sync();
+    meet();
   }
   ptx::grid_launch_dependents();
   if (p.behind_zeros) ptx::grid_wait_prerequisites();
@@ -673,14 +687,16 @@ int most_sorting_ctas() {
   return most;
 }
 
-// A token a thread up to the largest cluster, then 2, 4 or 8 a thread in
-// registers, then any number.
+// One CTA takes up to 2048 tokens (8.2 us for two passes of 2000; two CTAs 8.7,
+// but four CTAs 9.0 and one 12.7 for 4000), then a token a thread up to the
+// largest cluster, then 2, 4 or 8 a thread in registers, then any number.
+constexpr int kOneCta = 2 * kSortThreads;
 template <typename Id>
 int sort_any(const SortParams &p, cudaStream_t stream) {
   const int most = most_sorting_ctas();
   if (most == 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
   int cluster = 1;
-  while (cluster < most && p.n > kSortThreads * cluster) cluster *= 2;
+  while (p.n > kOneCta && cluster < most && p.n > kSortThreads * cluster) cluster *= 2;
   const int each = (p.n + cluster - 1) / cluster;
   if (each <= kSortThreads) return sort_ids<Id, 1>(p, cluster, stream);
   if (each <= 2 * kSortThreads) return sort_ids<Id, 2>(p, cluster, stream);

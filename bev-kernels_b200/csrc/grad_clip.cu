@@ -14,6 +14,13 @@
 // The tensors are cut into tiles of one size (a tensor's last one is shorter)
 // and every CTA takes a contiguous run of tiles.  Squares are summed in fp32
 // within a tile and thread, and those sums in fp64 in a fixed order.
+//
+// Bound by memory: 68 M bf16 elements clipped into fp32 take 97 us on the device
+// (136 MB read twice, 272 MB written: 5.6 TB/s), 28 us of it the norm, whose rate
+// grows from 4.8 TB/s at this size to 7.2 at 4 GB.  40 tensors of 1.3 M elements
+// within the limit take 6 us: launch, one round trip to memory, the grid's
+// meeting.  Keeping 192 KB a CTA pair in flight through asynchronous copies that
+// run on across tiles measured 109 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -13,8 +13,8 @@
 // Both directions are two sweeps over the same data with a reduction between
 // them: 2 (forward) or 3 (backward) passes over the tensor are what HBM has
 // to carry, so they are bound by memory once the tensors are large and by the
-// launch and the reduction's latency when they are small.  One cooperative
-// launch does both sweeps.  Every CTA owns a slab of pixels of one image (all
+// launch and the reduction's latency when they are small.  One launch does both
+// sweeps (cooperative, unless an image's CTAs make one cluster).  Every CTA owns a slab of pixels of one image (all
 // channels where C allows): consecutive threads take consecutive 16-byte
 // channel vectors, so a warp reads whole lines, and a thread keeps the same
 // channels throughout (its weights stay in registers).  After the first sweep
@@ -34,6 +34,16 @@
 // mean, M2) are joined by taking the mean of the means and then the squared
 // deviations from it.  That holds when the mean is far from zero and when
 // single values are far out.
+//
+// Device time, forward / backward (inputs in L2 where they fit; 16-bit unless
+// said; bytes are the 2 and 3 passes): 1x64x32x32 fp32 ReLU 6.4 us; 6x512x29x50
+// ReLU 9.8 (1.8 TB/s) / 16.8; 6x256x58x100 SiLU 14.2 / 28 us (2.5 / 1.9 TB/s);
+// 1x256x200x200 fp32 SiLU 19.7 / 45 us (4.2 / 2.7); 12x256x116x200 SiLU 94 / 174 us
+// (3.0 / 2.5).  The small ones are the latency of launch, load, reduction, meeting
+// and store, about 1 to 1.5 us each.  In the large ones a wave's meeting waits for
+// the stores of the wave before (2 to 3 us) and its partial results for the loads
+// in flight, and between those the SMs, 16 warps each, are at the instruction
+// rate of the activation.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
