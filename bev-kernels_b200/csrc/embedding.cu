@@ -105,6 +105,11 @@ __host__ __device__ constexpr Entry entry_of(unsigned key, unsigned pos) {
 }
 __device__ __forceinline__ unsigned key_in(Entry e) { return static_cast<unsigned>(e >> 32); }
 
+struct ZeroParams {  // zeros of a dense gradient: rows of row_bytes at pitch bytes
+  char *out;
+  int64_t rows, row_bytes, pitch;
+};
+
 struct SortParams {
   const void *ids;
   Entry *list0, *list1;  // written by the even and the odd passes
@@ -112,11 +117,7 @@ struct SortParams {
   int64_t rows, padding;
   int n, passes, cluster;
   int behind_zeros;   // launched while embedding_zero_kernel runs
-};
-
-struct ZeroParams {  // zeros of a dense gradient: rows of row_bytes at pitch bytes
-  char *out;
-  int64_t rows, row_bytes, pitch;
+  ZeroParams zeros;   // of a table that is small enough to leave them to the sort (rows > 0)
 };
 
 // An id as a sort key; what gets no gradient sorts behind all rows.
@@ -127,17 +128,8 @@ __device__ __forceinline__ unsigned key_of(Id id, const SortParams &p) {
                                                 : static_cast<unsigned>(p.rows);
 }
 
-constexpr int kZeroThreads = 512;
-
-// The zeros of a dense gradient, most of its bytes.  The sort needs few SMs and
-// waits for memory most of the time, so it runs at the same time: every CTA
-// here lets it start once the kernels before this one are complete, and the
-// sort waits for this kernel before it ends.
-__global__ void __launch_bounds__(kZeroThreads) embedding_zero_kernel(const ZeroParams p) {
-  ptx::grid_wait_prerequisites();
-  ptx::grid_launch_dependents();
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kZeroThreads + threadIdx.x;
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * kZeroThreads;
+// Writes thread `t` of `threads`' share of the zeros.
+__device__ __forceinline__ void write_zeros(const ZeroParams &p, int64_t t, int64_t threads) {
   const bool flat = p.row_bytes == p.pitch;
   const int64_t rows = flat ? 1 : p.rows;
   const int64_t bytes = flat ? p.rows * p.row_bytes : p.row_bytes;
@@ -155,6 +147,19 @@ __global__ void __launch_bounds__(kZeroThreads) embedding_zero_kernel(const Zero
       *reinterpret_cast<uint16_t *>(p.out + r * p.pitch + (i - r * halves) * 2) = 0;
     }
   }
+}
+
+constexpr int kZeroThreads = 512;
+
+// The zeros of a large dense gradient, most of its bytes.  The sort needs few
+// SMs and waits for memory most of the time, so it runs at the same time: every
+// CTA here lets it start once the kernels before this one are complete, and the
+// sort waits for this kernel before it ends.
+__global__ void __launch_bounds__(kZeroThreads) embedding_zero_kernel(const ZeroParams p) {
+  ptx::grid_wait_prerequisites();
+  ptx::grid_launch_dependents();
+  write_zeros(p, static_cast<int64_t>(blockIdx.x) * kZeroThreads + threadIdx.x,
+              static_cast<int64_t>(gridDim.x) * kZeroThreads);
 }
 
 // Inclusive sum over the warp's lanes.
@@ -209,6 +214,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
   const int chunk = ((b1 - b0 + kSortThreads - 1) / kSortThreads) * 32;
   const int w0 = min(b1, b0 + warp * chunk), w1 = min(b1, w0 + chunk);
   const Id *ids = static_cast<const Id *>(p.ids);
+  if (p.zeros.rows > 0)
+    write_zeros(p.zeros, rank * kSortThreads + tid, p.cluster * kSortThreads);
   const unsigned below = (1u << lane) - 1;
   // a cluster of one CTA spares itself the wider barrier's fence
   const auto meet = [&] {
@@ -790,16 +797,24 @@ int launch_embedding_backward(const bevk_embedding_backward_args *a, const void 
     const int64_t size = dtype_size(a->grad_table_dtype);
     const ZeroParams z = {static_cast<char *>(grad_table), a->num_rows, a->dim * size,
                           a->grad_table_ld * size};
-    const int64_t want = (z.rows * z.row_bytes + 64 * kZeroThreads - 1) / (64 * kZeroThreads);
-    const int dev = current_device();
-    if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
-    const int64_t most = int64_t(2) * device_info(dev).sm_count;  // leaves the sort room
-    st = launched(launch_dependent(embedding_zero_kernel,
-                                   dim3(static_cast<unsigned>(std::min(want, most))),
-                                   dim3(kZeroThreads), 0, stream, z),
-                  "embedding_zero_kernel");
-    if (st != BEVK_OK) return st;
-    s.behind_zeros = programmatic_launch_enabled();
+    const int64_t bytes = z.rows * z.row_bytes;
+    // four stores of every sorting thread cost less than a launch
+    const int64_t few = std::max<int64_t>(1, std::min<int64_t>(8, s.n / kSortThreads)) *
+                        kSortThreads * 64;
+    if (bytes <= few) {
+      s.zeros = z;
+    } else {
+      const int64_t want = (bytes + 64 * kZeroThreads - 1) / (64 * kZeroThreads);
+      const int dev = current_device();
+      if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
+      const int64_t most = int64_t(2) * device_info(dev).sm_count;  // leaves the sort room
+      st = launched(launch_dependent(embedding_zero_kernel,
+                                     dim3(static_cast<unsigned>(std::min(want, most))),
+                                     dim3(kZeroThreads), 0, stream, z),
+                    "embedding_zero_kernel");
+      if (st != BEVK_OK) return st;
+      s.behind_zeros = programmatic_launch_enabled();
+    }
   }
   st = a->ids_are_64bit ? sort_any<int64_t>(s, stream) : sort_any<int32_t>(s, stream);
   if (st != BEVK_OK) return st;

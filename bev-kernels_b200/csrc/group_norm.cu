@@ -160,13 +160,12 @@ __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
     return vio::two(sx, sy);
   } else {
     const float ex = exp2_approx(fminf(t.x, 125.f)), ey = exp2_approx(fminf(t.y, 125.f));
-    const vio::Two one = vio::two(1.f);
-    const vio::Two d = vio::add2(vio::two(ex, ey), one);
-    const float2 df = vio::split(d);
-    constexpr int kGuess = 0x7ef311c3;  // (254 - s) 2^23
-    const vio::Two minus = vio::two(-df.x, -df.y);
-    vio::Two y = vio::two(__int_as_float(kGuess - __float_as_int(df.x)),
-                          __int_as_float(kGuess - __float_as_int(df.y)));
+    // -d, whose sign bit the guess's constant takes off again
+    const vio::Two one = vio::two(1.f), minus = vio::fma2(vio::two(ex, ey), vio::two(-1.f), vio::two(-1.f));
+    const float2 m = vio::split(minus);
+    constexpr unsigned kGuess = 0x7ef311c3u + 0x80000000u;  // (254 - s) 2^23, and the sign
+    vio::Two y = vio::two(__uint_as_float(kGuess - __float_as_uint(m.x)),
+                          __uint_as_float(kGuess - __float_as_uint(m.y)));
     const vio::Two h = vio::fma2(minus, y, one);
     y = vio::fma2(y, vio::fma2(h, h, h), y);
     return vio::fma2(y, vio::fma2(minus, y, one), y);
@@ -469,7 +468,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
           const float2 s2 = vio::split(sum2[NC == 1 ? 0 : k / 2]), q2 = vio::split(sq2[NC == 1 ? 0 : k / 2]);
           const float sum = VEC == 1 ? s2.x : NC == 1 ? s2.x + s2.y : k % 2 ? s2.y : s2.x;
           const float sq = VEC == 1 ? q2.x : NC == 1 ? q2.x + q2.y : k % 2 ? q2.y : q2.x;
-          const float m2 = sq - sum * (sum * inv);
+          // squares that overflow leave an infinite variance, not a NaN
+          const float m2 = isinf(sq) ? sq : sq - sum * (sum * inv);
           s_red[(k * p.lanes + t.lane) * pitch + t.r] =
               make_float2(pivot[k] + sum * inv, m2 < 0.f ? 0.f : m2);
         }

@@ -171,6 +171,21 @@ def test_single_huge_value_and_nonfinite_stay_in_their_group(cuda):
     assert torch.equal(torch.isfinite(mean2), ~bad)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("c", [32, 21])
+def test_squares_past_the_range_of_fp32(cuda, dt, c):
+    """Deviations whose squares overflow: an infinite variance, so rstd is 0, the
+    output is act(bias) and grad_input 0 -- what the formulas give in fp32."""
+    x, gy, w, b = inputs(13, (1, c, 40, 30), dt, torch.float32, cuda)
+    x = x * 1e25
+    y, mean, rstd = gna.group_norm_act_forward(x, 1, w, b, EPS, "silu")
+    assert not rstd.any() and bool(torch.isfinite(mean).all())
+    want = torch.nn.functional.silu(b.double()).view(1, c, 1, 1).expand(y.shape)
+    assert rel_l2(y, want) <= UNIT[dt] + 16 * U32
+    gi, gw, gb = gna.group_norm_act_backward(gy, x, mean, rstd, 1, w, b, "silu")
+    assert not gi.any() and not gw.any() and bool(torch.isfinite(gb).all())
+
+
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 def test_layouts(cuda, dt):
     """Channels-last, a channel slice of a wider tensor (aligned or not), a crop,
