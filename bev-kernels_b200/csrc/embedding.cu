@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
     Entry *out = pass & 1 ? p.list1 : p.list0;
     const int shift = 32 + 8 * pass;
     const auto load = [&](int i) {
-      return pass ? __ldcg(in + i) : entry_of(key_of(ids[i], p), static_cast<unsigned>(i));
+      // from L2: what an SM may have cached is older than this kernel's start
+      return pass ? __ldcg(in + i) : entry_of(key_of(__ldcg(ids + i), p), static_cast<unsigned>(i));
     };
     const auto digit = [&](Entry e) { return static_cast<unsigned>(e >> shift) & (kDigits - 1); };
     Entry item[N];
