@@ -69,23 +69,35 @@ __global__ void __launch_bounds__(kLookThreads) embedding_forward_kernel(const L
       id[k] = r < p.n ? static_cast<int64_t>(ids[r]) : -1;
       if (id[k] >= p.rows) id[k] = -1;
     }
-    for (int c = tx * VEC; c < p.dim; c += p.tx * VEC) {
-      float v[kLookRows][VEC];
+    // single elements are taken four at a time, so that as many loads are on
+    // their way
+    constexpr int W = VEC == 1 ? 4 : 1;
+    for (int c0 = tx * VEC; c0 < p.dim; c0 += p.tx * VEC * W) {
+      float v[kLookRows][W][VEC];
 #pragma unroll
       for (int k = 0; k < kLookRows; ++k) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[k][e] = 0.f;
-        if (id[k] >= 0) vio::unpack(vio::load_pack<T, VEC>(table + id[k] * p.ld + c), v[k]);
+        for (int w = 0; w < W; ++w) {
+          const int c = c0 + w * p.tx;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[k][w][e] = 0.f;
+          if (id[k] >= 0 && c < p.dim)
+            vio::unpack(vio::load_pack<T, VEC>(table + id[k] * p.ld + c), v[k][w]);
+        }
       }
 #pragma unroll
       for (int k = 0; k < kLookRows; ++k) {
         const int64_t r = base + k * step + ty;
         if (r >= p.n) continue;
-        if (id[k] >= 0) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[k][e] *= p.scale;
+        for (int w = 0; w < W; ++w) {
+          const int c = c0 + w * p.tx;
+          if (id[k] >= 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[k][w][e] *= p.scale;
+          }
+          if (c < p.dim) vio::store<T, VEC>(out + r * p.dim + c, v[k][w]);
         }
-        vio::store<T, VEC>(out + r * p.dim + c, v[k]);
       }
     }
   }
@@ -128,22 +140,30 @@ __device__ __forceinline__ unsigned key_of(Id id, const SortParams &p) {
                                                 : static_cast<unsigned>(p.rows);
 }
 
-// Writes thread `t` of `threads`' share of the zeros.
+// Writes thread `t` of `threads`' share of the zeros: 16 bytes at a time in one
+// stretch of memory (its ends by halves: elements have two bytes at least) or in
+// rows of whole 16-byte parts, else halves.
 __device__ __forceinline__ void write_zeros(const ZeroParams &p, int64_t t, int64_t threads) {
-  const bool flat = p.row_bytes == p.pitch;
-  const int64_t rows = flat ? 1 : p.rows;
-  const int64_t bytes = flat ? p.rows * p.row_bytes : p.row_bytes;
-  if (reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && bytes % 16 == 0 &&
-      (flat || p.pitch % 16 == 0)) {
-    const int64_t vecs = bytes / 16;
-    for (int64_t i = t; i < rows * vecs; i += threads) {
-      const int64_t r = flat ? 0 : i / vecs;
-      *reinterpret_cast<uint4 *>(p.out + r * p.pitch + (i - r * vecs) * 16) = make_uint4(0, 0, 0, 0);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if (p.row_bytes == p.pitch || p.rows == 1) {
+    const int64_t bytes = p.rows * p.row_bytes;
+    const int64_t head = min(bytes, static_cast<int64_t>(-reinterpret_cast<uintptr_t>(p.out) & 15));
+    const int64_t vecs = (bytes - head) / 16, tail = head + vecs * 16;
+    for (int64_t i = t; i < vecs; i += threads)
+      *reinterpret_cast<uint4 *>(p.out + head + i * 16) = zero;
+    if (2 * t < head) *reinterpret_cast<uint16_t *>(p.out + 2 * t) = 0;
+    if (2 * t < bytes - tail) *reinterpret_cast<uint16_t *>(p.out + tail + 2 * t) = 0;
+  } else if (reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.row_bytes % 16 == 0 &&
+             p.pitch % 16 == 0) {
+    const int64_t vecs = p.row_bytes / 16;
+    for (int64_t i = t; i < p.rows * vecs; i += threads) {
+      const int64_t r = i / vecs;
+      *reinterpret_cast<uint4 *>(p.out + r * p.pitch + (i - r * vecs) * 16) = zero;
     }
-  } else {  // elements of two bytes at least
-    const int64_t halves = bytes / 2;
-    for (int64_t i = t; i < rows * halves; i += threads) {
-      const int64_t r = flat ? 0 : i / halves;
+  } else {
+    const int64_t halves = p.row_bytes / 2;
+    for (int64_t i = t; i < p.rows * halves; i += threads) {
+      const int64_t r = i / halves;
       *reinterpret_cast<uint16_t *>(p.out + r * p.pitch + (i - r * halves) * 2) = 0;
     }
   }
@@ -380,16 +400,23 @@ constexpr int kSumThreads = 256;
 // Rows on their way per warp: every thread copies its part of them asynchronously
 // into slots of its own in shared memory, so the loop over the tile's tokens is
 // short and a warp waits for its next row only.  (Parts of two bytes, which
-// cannot be copied so, are loaded kAhead at a time instead.)  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with 16
+// cannot be copied so, are loaded kBatch rows and kWide columns at a time instead.)  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with 16
 // rows and 3 CTAs per SM, 104 to 108 with 4 to 24 rows and 8 to 2, and with
 // batches of 16 rows in registers.
 constexpr int kAhead = 16;
+constexpr int kBatch = 8, kWide = 4;
 
-// One warp per (tile, slice of 32 * VEC columns).
+// Columns that a warp takes of a tile: 32 of VEC each, or kWide times 32 of two
+// bytes.
+template <typename T, int VEC>
+constexpr int kSliceColumns = 32 * VEC * (sizeof(T) * VEC >= 4 ? 1 : kWide);
+
+// One warp per (tile, slice of the columns).
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const SumParams p) {
   constexpr int kBytes = sizeof(T) * VEC;
   constexpr bool kAsync = kBytes >= 4;
+  constexpr int W = kAsync ? 1 : kWide;  // a thread's columns are c + 32 w (+ VEC)
   constexpr int kSlot = 32 * kBytes;
   extern __shared__ float4 s_dyn[];  // [warp][kAhead][lane] where copies are asynchronous
   ptx::grid_launch_dependents();
@@ -397,7 +424,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kSumThreads / 32) + (threadIdx.x >> 5);
   const int64_t tile = item / p.slices;
-  const int c = (static_cast<int>(item - tile * p.slices) * 32 + lane) * VEC;
+  const int c = static_cast<int>(item - tile * p.slices) * kSliceColumns<T, VEC> + lane * VEC;
   const int64_t first = tile * kTile;
   if (first >= p.n) return;
   const Entry none = entry_of(static_cast<unsigned>(p.rows), 0);
@@ -424,34 +451,43 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
 #pragma unroll 4
     for (int t = 0; t < kAhead; ++t) fetch(t);
   }
-  float acc[VEC];
+  float acc[W][VEC];
+  const auto clear = [&] {
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[w][k] = 0.f;
+  };
+  clear();
   int begin = 0;
-  vio::Pack<T, VEC> batch[kAsync ? 1 : kAhead];
+  vio::Pack<T, VEC> batch[kAsync ? 1 : kBatch][W];
 #pragma unroll 1
   for (int t = 0; t < count; ++t) {
-    vio::Pack<T, VEC> q;
     if constexpr (!kAsync) {
-      if (t % kAhead == 0) {
+      if (t % kBatch == 0) {
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
+        for (int j = 0; j < kBatch; ++j) {
           const T *src = row_of(t + j);
-          if (col && t + j < count) batch[j] = vio::load_pack<T, VEC>(src);
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (c + 32 * w < p.dim && t + j < count)
+              batch[j][w] = vio::load_pack<T, VEC>(src + 32 * w);
         }
       }
-      q = batch[0];
-#pragma unroll
-      for (int j = 0; j + 1 < kAhead; ++j) batch[j] = batch[j + 1];
     } else {
       asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-      q = vio::load_pack<T, VEC>(ring + t % kAhead * kSlot);
+      batch[0][0] = vio::load_pack<T, VEC>(ring + t % kAhead * kSlot);
     }
-    if (col) {
-      float v[VEC];
-      vio::unpack(q, v);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    for (int w = 0; w < W; ++w) {
+      float v[VEC];
+      vio::unpack(batch[0][w], v);
+      if (c + 32 * w < p.dim) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[w][k] += v[k];
+      }
+#pragma unroll
+      for (int j = 0; j + 1 < (kAsync ? 1 : kBatch); ++j) batch[j][w] = batch[j + 1][w];
     }
     if constexpr (kAsync) fetch(t + kAhead);
     if (!((ends >> t) & 1u)) continue;
@@ -465,24 +501,26 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
       const unsigned at = atomicAdd(p.count + (is_long ? 1 : 0), 1u);
       (is_long ? p.owner1 : p.owner0)[at] = static_cast<unsigned>(2 * tile + (begin ? 1 : 0));
     }
-    if (col) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int cw = c + 32 * w;
+      if (cw >= p.dim) continue;
       if (open) {
-        float *dst = p.partial + (tile * 2 + (begin ? 1 : 0)) * p.pdim + c;
+        float *dst = p.partial + (tile * 2 + (begin ? 1 : 0)) * p.pdim + cw;
         if constexpr (VEC % 4 == 0) {
 #pragma unroll
           for (int k = 0; k < VEC; k += 4)
             __stcg(reinterpret_cast<float4 *>(dst + k),
-                   make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]));
+                   make_float4(acc[w][k], acc[w][k + 1], acc[w][k + 2], acc[w][k + 3]));
         } else {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) __stcg(dst + k, acc[k]);
+          for (int k = 0; k < VEC; ++k) __stcg(dst + k, acc[w][k]);
         }
       } else {
-        finish<O, VEC>(p, row, c, acc);
+        finish<O, VEC>(p, row, cw, acc[w]);
       }
     }
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    clear();
     begin = t + 1;
   }
 }
@@ -716,7 +754,7 @@ int sort_any(const SortParams &p, cudaStream_t stream) {
 template <typename T, typename O, int VEC>
 int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
   SumParams p = p0;
-  p.slices = (p.dim + 32 * VEC - 1) / (32 * VEC);
+  p.slices = (p.dim + kSliceColumns<T, VEC> - 1) / kSliceColumns<T, VEC>;
   const int64_t warps = tiles * p.slices, per = kSumThreads / 32;
   const int64_t grid = (warps + per - 1) / per;
   if (grid >= (int64_t(1) << 31))

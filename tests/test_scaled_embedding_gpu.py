@@ -251,3 +251,41 @@ def test_refusals(cuda):
         emb.scaled_embedding_backward(gy, ids, 5, grad_weight=torch.zeros(8, 5, device=cuda).t())
     with pytest.raises(RuntimeError, match="dtypes"):
         emb.scaled_embedding_backward(gy, ids, 5, grad_weight=w.half())
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,dim", [(7, 3), (1000, 5), (12450, 37), (1, 1), (333, 2049)])
+def test_zeros_of_odd_tables(cuda, rows, dim, dt):
+    """Rows that no id names are zero, whatever the table's size in bytes, and
+    nothing is written beside the table."""
+    ids = torch.tensor([0], device=cuda)
+    gy = torch.ones(1, dim, device=cuda, dtype=dt)
+    for _ in range(2):
+        torch.full((rows * dim + 4096,), float("nan"), device=cuda, dtype=dt)  # what the memory may hold
+        grad = emb.scaled_embedding_backward(gy, ids, rows)
+        assert bool((grad[0] == 1).all()) and not grad[1:].any()
+
+
+def test_dense_gradient_into_a_wider_buffer(cuda):
+    """The C ABI's row stride: zeros go to the rows only."""
+    import ctypes
+
+    from bevk import cabi
+    L = cabi.lib()
+    for dim, ld, at in ((24, 40, 0), (24, 25, 0), (23, 40, 1)):
+        buf = torch.full((50 * ld + at,), 7.0, device=cuda)
+        ids = torch.tensor([3, 3, 49], device=cuda)
+        gy = torch.ones(3, dim, device=cuda)
+        a = cabi.EmbeddingBackwardArgs()
+        a.num_ids, a.num_rows, a.dim, a.ids_are_64bit = 3, 50, dim, 1
+        a.grad_output_ld, a.grad_table_ld, a.padding_idx, a.scale = dim, ld, -1, 1.0
+        n = L.bevk_embedding_backward_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty(n, dtype=torch.uint8, device=cuda)
+        cabi.check(L.bevk_embedding_backward(
+            ctypes.byref(a), gy.data_ptr(), ids.data_ptr(), buf.data_ptr() + 4 * at, ws.data_ptr(), n,
+            torch.cuda.current_stream().cuda_stream), "embedding_backward")
+        rows = buf[at:].view(50, ld)
+        assert bool((rows[:, dim:] == 7).all()) and bool((buf[:at] == 7).all())
+        want = torch.zeros(50, dim, device=cuda)
+        want[3], want[49] = 2, 1
+        assert torch.equal(rows[:, :dim], want)
