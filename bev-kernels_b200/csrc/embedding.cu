@@ -400,8 +400,9 @@ constexpr int kSumThreads = 256;
 // Rows on their way per warp: every thread copies its part of them asynchronously
 // into slots of its own in shared memory, so the loop over the tile's tokens is
 // short and a warp waits for its next row only.  (Parts of two bytes, which
-// cannot be copied so, are loaded kBatch rows and kWide columns at a time instead.)  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with 16
-// rows and 3 CTAs per SM, 104 to 108 with 4 to 24 rows and 8 to 2, and with
+// cannot be copied so, are loaded kBatch rows and kWide columns at a time
+// instead.)  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with
+// 16 rows and 3 CTAs per SM, 104 to 108 with 4 to 24 rows and 8 to 2, and with
 // batches of 16 rows in registers.
 constexpr int kAhead = 16;
 constexpr int kBatch = 8, kWide = 4;

@@ -14,13 +14,13 @@
 // them: 2 (forward) or 3 (backward) passes over the tensor are what HBM has
 // to carry, so they are bound by memory once the tensors are large and by the
 // launch and the reduction's latency when they are small.  One launch does both
-// sweeps (cooperative, unless an image's CTAs make one cluster).  Every CTA owns a slab of pixels of one image (all
-// channels where C allows): consecutive threads take consecutive 16-byte
-// channel vectors, so a warp reads whole lines, and a thread keeps the same
-// channels throughout (its weights stay in registers).  After the first sweep
-// each CTA leaves one partial result per group, the grid meets, and each CTA
-// joins the partials of its own image in a fixed order before its second
-// sweep.
+// sweeps (cooperative, unless an image's CTAs make one cluster).  Every CTA owns
+// a slab of pixels of one image (all channels where C allows): consecutive
+// threads take consecutive 16-byte channel vectors, so a warp reads whole lines,
+// and a thread keeps the same channels throughout (its weights stay in
+// registers).  After the first sweep each CTA leaves one partial result per
+// group, the CTAs meet, and each joins the partials of its own image in a fixed
+// order before its second sweep.
 //
 // Every thread copies its own vectors to shared memory asynchronously -- all
 // of them at once, without registers, and without synchronising with other
@@ -162,7 +162,8 @@ __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
   } else {
     const float ex = exp2_approx(fminf(t.x, 125.f)), ey = exp2_approx(fminf(t.y, 125.f));
     // -d, whose sign bit the guess's constant takes off again
-    const vio::Two one = vio::two(1.f), minus = vio::fma2(vio::two(ex, ey), vio::two(-1.f), vio::two(-1.f));
+    const vio::Two one = vio::two(1.f);
+    const vio::Two minus = vio::fma2(vio::two(ex, ey), vio::two(-1.f), vio::two(-1.f));
     const float2 m = vio::split(minus);
     constexpr unsigned kGuess = 0x7ef311c3u + 0x80000000u;  // (254 - s) 2^23, and the sign
     vio::Two y = vio::two(__uint_as_float(kGuess - __float_as_uint(m.x)),
@@ -391,7 +392,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
   const Place t = place<VEC>(p);
   const int held = min(t.mine, p.keep);
   const int groups = (p.keep + kBatch - 1) / kBatch;  // asynchronous ones, of every thread
-  const int64_t hop = static_cast<int64_t>(p.R) * p.xs[1], out_hop = static_cast<int64_t>(p.R) * p.os[1];
+  const int64_t hop = static_cast<int64_t>(p.R) * p.xs[1];
+  const int64_t out_hop = static_cast<int64_t>(p.R) * p.os[1];
   int n = t.image;
   const T *src = static_cast<const T *>(p.x) + n * p.xs[0] +
                  static_cast<int64_t>(t.p0 + t.r) * p.xs[1] + t.c;
@@ -425,7 +427,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
         for (int k = 0; k < NC; ++k) pivot[k] *= inv;
 #pragma unroll
         for (int k = 0; k < (NC == 1 ? 1 : P); ++k)
-          minus[k] = vio::two(-pivot[NC == 1 ? 0 : 2 * k], VEC == 1 ? 0.f : -pivot[NC == 1 ? 0 : 2 * k + 1]);
+          minus[k] = vio::two(-pivot[NC == 1 ? 0 : 2 * k],
+                              VEC == 1 ? 0.f : -pivot[NC == 1 ? 0 : 2 * k + 1]);
       };
       const auto add = [&](const Vec &q) {
         vio::Two f[P];
@@ -466,7 +469,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
         const float inv = reciprocal(static_cast<float>(max(t.mine, 1) * CH));
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
-          const float2 s2 = vio::split(sum2[NC == 1 ? 0 : k / 2]), q2 = vio::split(sq2[NC == 1 ? 0 : k / 2]);
+          const float2 s2 = vio::split(sum2[NC == 1 ? 0 : k / 2]);
+          const float2 q2 = vio::split(sq2[NC == 1 ? 0 : k / 2]);
           const float sum = VEC == 1 ? s2.x : NC == 1 ? s2.x + s2.y : k % 2 ? s2.y : s2.x;
           const float sq = VEC == 1 ? q2.x : NC == 1 ? q2.x + q2.y : k % 2 ? q2.y : q2.x;
           // squares that overflow leave an infinite variance, not a NaN
@@ -510,14 +514,17 @@ __global__ void __launch_bounds__(kForwardThreads, 1)
         if (gl < t.ng && j == 0) __stcg(partial_slot(p, t, n, gl), make_float2(mean, m2));
       }
     }
-    const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
-    const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
+    const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype,
+                                           p.param_vectors != 0);
+    const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype,
+                                           p.param_vectors != 0);
     if (p.S == 1 && p.nb == 1) __syncthreads();
     else if (p.cluster) ptx::cluster_sync();
     else grid.sync();
     const bool next = n + p.wave < p.N;
     if (n < p.N) {
-      combine_moments<kThreads>(p, t, n, p.lanes * VEC, s_mean, s_rstd, p.mean != nullptr && t.s == 0);
+      combine_moments<kThreads>(p, t, n, p.lanes * VEC, s_mean, s_rstd,
+                                p.mean != nullptr && t.s == 0);
       __syncthreads();
       float a[VEC], b[VEC];  // z = a x + b
       vio::params_to_float(pw, p.w, p.param_dtype, 1.f, a);
@@ -606,8 +613,10 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
   }
   float w[VEC], b[VEC];
   {
-    const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
-    const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype, p.param_vectors != 0);
+    const auto pw = vio::load_params<VEC>(t.active ? p.w : nullptr, t.c, p.param_dtype,
+                                           p.param_vectors != 0);
+    const auto pb = vio::load_params<VEC>(t.active ? p.b : nullptr, t.c, p.param_dtype,
+                                           p.param_vectors != 0);
     vio::params_to_float(pw, p.w, p.param_dtype, 1.f, w);
     vio::params_to_float(pb, p.b, p.param_dtype, 0.f, b);
   }

@@ -174,7 +174,8 @@ __device__ __forceinline__ void unpack2(const Pack<T, VEC> &q, Two (&f)[kPairsOf
 #pragma unroll
   for (int i = 0; i < kPairsOf<VEC>; ++i) {
     if constexpr (sizeof(T) == 4) {
-      f[i] = two(__uint_as_float(q.w[2 * i]), VEC == 1 ? 0.f : __uint_as_float(q.w[VEC == 1 ? 0 : 2 * i + 1]));
+      f[i] = two(__uint_as_float(q.w[2 * i]),
+                 VEC == 1 ? 0.f : __uint_as_float(q.w[VEC == 1 ? 0 : 2 * i + 1]));
     } else {
       const float2 v = widen2(q.w[i], T());
       f[i] = two(v.x, VEC == 1 ? 0.f : v.y);
@@ -197,14 +198,7 @@ __device__ __forceinline__ void store2(T *p, const Two (&f)[kPairsOf<VEC>]) {
   store_pack<T, VEC>(p, q);
 }
 
-// A scalar of the parameter type chosen at run time (fp32, fp16 or bf16).
-__device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
-  switch (dtype) {
-    case 1: return __half2float(static_cast<const __half *>(p)[i]);
-    case 2: return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-    default: return static_cast<const float *>(p)[i];
-  }
-}
+// Stores a scalar as the type chosen at run time (fp32, fp16 or bf16).
 __device__ __forceinline__ void store_any(void *p, int64_t i, int dtype, float v) {
   switch (dtype) {
     case 1: static_cast<__half *>(p)[i] = __float2half_rn(v); break;

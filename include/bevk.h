@@ -93,6 +93,8 @@ BEVK_API int bevk_set_wait_limit_ns(int device, unsigned long long ns);
  * waits for it to complete before reading or writing global memory, so stream
  * order holds as with ordinary launches.  Setting the environment variable
  * BEVK_PDL=0 (read once per process) launches them the ordinary way.
+ * (Cooperative launches -- group norm and gradient clipping -- always are
+ * ordinary ones.)
  */
 
 /* ------------------------------------------------------------------------ */
