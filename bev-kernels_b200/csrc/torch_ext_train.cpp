@@ -22,6 +22,13 @@ using OptTensor = std::optional<Tensor>;
 // that the extension was built with.
 std::string str(int64_t v) { return std::to_string(v); }
 
+// Counts a write through a tensor's pointer, as torch's own operators count theirs:
+// a graph that saved the tensor before then refuses the new values.  (Inference
+// tensors are not counted.)
+void count_write(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ------------------------------------------------------- group norm + act
 
 // Whether the tensor can be addressed as {image, pixel} strides with channel
@@ -348,6 +355,8 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
                               current_stream(first)),
                "grad_clip");
   for (auto &c : copy_back) c.first.copy_(c.second);
+  if (max_norm)
+    for (const Tensor &t : out ? *out : grads) count_write(t);
   return norm;
 }
 

@@ -12,7 +12,8 @@ tensors are on one GPU.  Nothing synchronises (``error_if_nonfinite=True``
 reads the norm and does).  A NaN gradient makes the norm and every output NaN;
 an infinite norm scales by zero.  Equal inputs give equal bits.  Tensors with
 holes between their elements are clipped through a dense copy.  A tensor may
-stand in the list once.
+stand in the list once.  Every written tensor counts a new version, whether or
+not its values change, so autograd refuses a graph that saved it before.
 """
 from __future__ import annotations
 

@@ -1,0 +1,55 @@
+"""What the training-side operators tell autograd: tensors that they write count
+a new version."""
+import pytest
+import torch
+
+import grad_clip
+
+pytestmark = pytest.mark.gpu
+
+
+def saved_gradient(device, shape=(6, 8)):
+    """A gradient that a graph has saved, and a loss over it."""
+    x = torch.randn(shape, generator=torch.Generator(device).manual_seed(0), device=device)
+    x.requires_grad_()
+    gx, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    return x, gx, (gx * gx).sum()
+
+
+@pytest.mark.parametrize("limit", [0.1, 1e9], ids=["scaled", "within the limit"])
+def test_clipping_counts_versions(cuda, limit):
+    wide = torch.ones(8, 12, device=cuda)
+    tensors = [torch.ones(5, device=cuda), torch.ones(3, 4, 5, device=cuda).permute(2, 0, 1),
+               wide[:, 3:7]]
+    before = [t._version for t in tensors]
+    grad_clip.grad_norm(tensors)
+    assert [t._version for t in tensors] == before               # only read
+    grad_clip.clip_grads(tensors, limit)
+    after = [t._version for t in tensors]
+    assert all(a > b for a, b in zip(after, before))
+    out = [torch.zeros_like(t) for t in tensors]
+    at = [o._version for o in out]
+    grad_clip.clip_grads(tensors, limit, out=out)
+    assert all(o._version > v for o, v in zip(out, at))
+    assert [t._version for t in tensors] == after                # read again
+    p = torch.nn.Parameter(torch.ones(4, device=cuda))
+    p.grad = torch.ones(4, device=cuda)
+    v = p.grad._version
+    grad_clip.clip_grad_norm_([p], limit)
+    assert p.grad._version > v and p._version == 0
+
+
+def test_a_graph_refuses_a_gradient_that_was_clipped_since(cuda):
+    x, gx, loss = saved_gradient(cuda)
+    grad_clip.clip_grads([gx], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_inference_tensors_are_written_as_before(cuda):
+    """They have no versions; torch's own operators refuse them outside of
+    inference mode, these never have."""
+    with torch.inference_mode():
+        g = torch.full((4,), 2.0, device=cuda)
+    assert float(grad_clip.clip_grads([g], 1.0)) == 4.0
+    assert float(g.double().norm()) == pytest.approx(1.0, rel=1e-5)
