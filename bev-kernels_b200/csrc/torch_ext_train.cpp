@@ -261,6 +261,7 @@ Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t
   check_status(bevk_embedding_backward(&a, dy.data_ptr(), ids.data_ptr(), out.data_ptr(),
                                        ws.get(), bytes, current_stream(grad_output)),
                "embedding_backward");
+  if (into) count_write(out);
   return out;
 }
 

@@ -53,7 +53,7 @@ def scaled_embedding_backward(grad_output: torch.Tensor, ids: torch.Tensor, num_
     """-> the weight's gradient [num_embeddings, dim] in grad_output's dtype, with
     zeros in the rows that no id names.  Where ``grad_weight`` (grad_output's dtype
     or fp32) is given, the gradient is added to it instead, in place, and it is
-    returned."""
+    returned; it counts a new version."""
     return _load_ext().embedding_backward(grad_output, ids, num_embeddings, scale,
                                           _padding(padding_idx, num_embeddings), grad_weight)
 

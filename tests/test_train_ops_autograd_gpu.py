@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import grad_clip
+import scaled_embedding as emb
 
 pytestmark = pytest.mark.gpu
 
@@ -46,6 +47,16 @@ def test_a_graph_refuses_a_gradient_that_was_clipped_since(cuda):
         loss.backward()
 
 
+def test_an_added_embedding_gradient_counts_versions(cuda):
+    ids = torch.tensor([0, 2, 2], device=cuda)
+    _, gx, loss = saved_gradient(cuda)
+    v = gx._version
+    emb.scaled_embedding_backward(torch.ones(3, 8, device=cuda), ids, 6, grad_weight=gx)
+    assert gx._version > v
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_inference_tensors_are_written_as_before(cuda):
     """They have no versions; torch's own operators refuse them outside of
     inference mode, these never have."""
@@ -53,3 +64,11 @@ def test_inference_tensors_are_written_as_before(cuda):
         g = torch.full((4,), 2.0, device=cuda)
     assert float(grad_clip.clip_grads([g], 1.0)) == 4.0
     assert float(g.double().norm()) == pytest.approx(1.0, rel=1e-5)
+
+
+def test_embedding_gradients_added_to_inference_tensors(cuda):
+    with torch.inference_mode():
+        main = torch.zeros(6, 8, device=cuda)
+    emb.scaled_embedding_backward(torch.ones(1, 8, device=cuda), torch.tensor([5], device=cuda), 6,
+                                  grad_weight=main)
+    assert float(main[5].sum()) == 8.0
