@@ -280,6 +280,7 @@ Tensor empty_dense(const Tensor &like, at::ScalarType dtype) {
 // their gradient's, go through a dense copy.
 Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_norm, double eps,
                  bool inf_norm, const std::optional<std::vector<Tensor>> &out) {
+  const at::NoGradGuard no_grad;  // the copies below are no part of the caller's graph
   TORCH_CHECK(!grads.empty(), "bevk: no gradients");
   TORCH_CHECK(!out || out->size() == grads.size(), "bevk: one output for each gradient");
   const Tensor &first = grads[0];

@@ -1,5 +1,6 @@
 """What the training-side operators tell autograd: tensors that they write count
-a new version."""
+a new version, and nothing that they do becomes part of a graph behind the
+caller's back."""
 import pytest
 import torch
 
@@ -72,3 +73,19 @@ def test_embedding_gradients_added_to_inference_tensors(cuda):
     emb.scaled_embedding_backward(torch.ones(1, 8, device=cuda), torch.tensor([5], device=cuda), 6,
                                   grad_weight=main)
     assert float(main[5].sum()) == 8.0
+
+
+def test_copies_for_gradients_with_holes_stay_out_of_the_graph(cuda):
+    """A clipped view of a gradient that is itself part of a graph: its values
+    change, its derivative is not replaced by that of the copies."""
+    x, gx, _ = saved_gradient(cuda)
+    view = gx[:, 2:5]
+    grad_clip.clip_grads([view], 0.1)
+    assert float(view.detach().double().norm()) == pytest.approx(0.1, rel=1e-5)
+    assert gx.grad_fn.name() != "CopySlices"
+    leaf = torch.ones(4, 6, device=cuda, requires_grad=True)     # a leaf, dense or through a copy
+    grad_clip.clip_grads([leaf], 1.0)
+    with torch.no_grad():
+        part = leaf[:, 1:3]
+    grad_clip.clip_grads([part], 0.5)
+    assert float(part.detach().double().norm()) == pytest.approx(0.5, rel=1e-5)
