@@ -29,6 +29,16 @@ void count_write(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// The operators have no forward-mode derivative.  A tangent is refused, as torch
+// refuses it for a Function without one: the result would have none, which reads
+// as a derivative of zero.  (In the forward of a custom Function forward mode is
+// off: what is called there has its derivative from the Function.)
+void check_no_tangent(const Tensor &t, const char *name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
+      "bevk: ", name, " has a forward-mode tangent; this operator has no forward-mode derivative");
+}
+
 // ------------------------------------------------------- group norm + act
 
 // Whether the tensor can be addressed as {image, pixel} strides with channel
@@ -82,6 +92,7 @@ bevk_group_norm_problem gn_problem(const Tensor &input, int64_t num_groups,
                                    const OptTensor &weight, const OptTensor &bias, double eps,
                                    int64_t act) {
   check_cuda(input, "input");
+  check_no_tangent(input, "input");
   TORCH_CHECK(input.dim() >= 2, "bevk: input must be [N, C, *spatial]");
   TORCH_CHECK(num_groups > 0 && input.size(1) > 0 && input.size(1) % num_groups == 0,
               "bevk: num_groups=", str(num_groups), " must divide the channels (",
@@ -95,6 +106,7 @@ bevk_group_norm_problem gn_problem(const Tensor &input, int64_t num_groups,
   for (const OptTensor *t : {&weight, &bias}) {
     if (!*t) continue;
     check_same_device(input, **t, "weight / bias");
+    check_no_tangent(**t, "weight / bias");
     TORCH_CHECK((*t)->dim() == 1 && (*t)->size(0) == input.size(1) && (*t)->is_contiguous(),
                 "bevk: weight and bias must be contiguous [C]");
     const int dt = dtype_of(**t);
@@ -149,8 +161,10 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(
     int64_t num_groups, const OptTensor &weight, const OptTensor &bias, int64_t act,
     bool need_input, bool need_weight, bool need_bias) {
   bevk_group_norm_problem p = gn_problem(input_, num_groups, weight, bias, 0.0, act);
-  for (const Tensor *t : {&grad_output_, &mean, &rstd})
+  for (const Tensor *t : {&grad_output_, &mean, &rstd}) {
     check_same_device(input_, *t, "group norm tensor");
+    check_no_tangent(*t, "group norm tensor");
+  }
   TORCH_CHECK(grad_output_.sizes() == input_.sizes() &&
                   grad_output_.scalar_type() == input_.scalar_type(),
               "bevk: grad_output must have input's shape and dtype");
@@ -200,6 +214,7 @@ int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.siz
 Tensor embedding_forward(const Tensor &table, const Tensor &ids_, double scale) {
   check_cuda(table, "weight");
   check_same_device(table, ids_, "ids");
+  check_no_tangent(table, "weight");
   TORCH_CHECK(table.dim() == 2 && table.size(1) > 0, "bevk: weight must be [rows, dim]");
   TORCH_CHECK(table.size(1) < (int64_t(1) << 24), "bevk: weight has too many columns");
   const bool wide = wide_ids(ids_);
@@ -222,6 +237,7 @@ Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t
                           double scale, int64_t padding_idx, const OptTensor &into) {
   check_cuda(grad_output, "grad_output");
   check_same_device(grad_output, ids_, "ids");
+  check_no_tangent(grad_output, "grad_output");
   const bool wide = wide_ids(ids_);
   TORCH_CHECK(grad_output.dim() == ids_.dim() + 1 &&
                   grad_output.sizes().slice(0, ids_.dim()) == ids_.sizes(),
@@ -237,6 +253,7 @@ Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t
   Tensor out;
   if (into) {
     check_same_device(grad_output, *into, "grad_weight");
+    check_no_tangent(*into, "grad_weight");
     TORCH_CHECK(into->dim() == 2 && into->size(0) == num_rows && into->size(1) == dim,
                 "bevk: grad_weight must be [num_embeddings, dim]");
     TORCH_CHECK((dim == 1 || into->stride(1) == 1) &&
@@ -296,6 +313,8 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
       check_same_device(first, g, "gradient");
     }
     TORCH_CHECK(g.layout() == at::kStrided, "bevk: gradients must be strided tensors");
+    check_no_tangent(g, "gradient");
+    if (max_norm && out) check_no_tangent((*out)[i], "output");
     bevk_grad_tensor &it = items[i];
     it.grad_dtype = dtype_of(g);
     it.numel = g.numel();

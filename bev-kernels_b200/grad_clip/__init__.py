@@ -14,6 +14,7 @@ an infinite norm scales by zero.  Equal inputs give equal bits.  Tensors with
 holes between their elements are clipped through a dense copy.  A tensor may
 stand in the list once.  Every written tensor counts a new version, whether or
 not its values change, so autograd refuses a graph that saved it before.
+Tensors with a forward-mode tangent raise NotImplementedError.
 """
 from __future__ import annotations
 

@@ -14,7 +14,8 @@ share its dtype or are fp32.  Statistics and sums are fp32 and the result is
 rounded once.  Channels-last memory (also with a wider pixel stride, e.g. a
 channel slice) is read in place, any other layout is first copied to it; the
 output and ``grad_input`` are channels-last.  ``act`` is "none", "relu" or
-"silu".  CUDA tensors only.
+"silu".  CUDA tensors only; there is no forward-mode derivative (a tangent
+raises NotImplementedError).
 """
 from __future__ import annotations
 

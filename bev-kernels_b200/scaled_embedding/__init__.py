@@ -11,7 +11,8 @@ ids are int64 or int32 of any shape; the table is fp32, fp16 or bf16.  An id
 outside [0, rows) reads as a row of zeros and gives no gradient; the row
 ``padding_idx`` is read as any other and gets no gradient.  Sums are fp32 and
 their order is fixed by the ids alone, so equal inputs give equal bits.  CUDA
-tensors only.
+tensors only; there is no forward-mode derivative (a tangent raises
+NotImplementedError).
 """
 from __future__ import annotations
 

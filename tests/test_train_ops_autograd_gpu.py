@@ -1,10 +1,12 @@
 """What the training-side operators tell autograd: tensors that they write count
-a new version, and nothing that they do becomes part of a graph behind the
-caller's back."""
+a new version, forward-mode tangents are refused instead of dropped, and nothing
+that they do becomes part of a graph behind the caller's back."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import grad_clip
+import group_norm_act as gna
 import scaled_embedding as emb
 
 pytestmark = pytest.mark.gpu
@@ -89,3 +91,62 @@ def test_copies_for_gradients_with_holes_stay_out_of_the_graph(cuda):
         part = leaf[:, 1:3]
     grad_clip.clip_grads([part], 0.5)
     assert float(part.detach().double().norm()) == pytest.approx(0.5, rel=1e-5)
+
+
+@pytest.mark.parametrize("grad_mode", [True, False], ids=["grad", "no_grad"])
+@pytest.mark.parametrize("which", [0, 1, 2], ids=["input", "weight", "bias"])
+def test_group_norm_refuses_tangents(cuda, grad_mode, which):
+    args = [torch.randn(2, 8, 3, 3, device=cuda), torch.ones(8, device=cuda),
+            torch.zeros(8, device=cuda)]
+    plain = gna.group_norm_act(args[0], 2, args[1], args[2], act="silu")
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        # without tangents the call is what it is outside
+        assert torch.equal(gna.group_norm_act(args[0], 2, args[1], args[2], act="silu"), plain)
+        dual = list(args)
+        dual[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError):
+            gna.group_norm_act(dual[0], 2, dual[1], dual[2], act="silu")
+        with pytest.raises(NotImplementedError):
+            gna.group_norm_act_forward(dual[0], 2, dual[1], dual[2], act="silu")
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda t: gna.group_norm_act(t, 2), (args[0],), (torch.ones_like(args[0]),))
+
+
+def test_the_other_operators_refuse_tangents(cuda):
+    x, w = torch.randn(2, 8, 3, 3, device=cuda), torch.randn(5, 8, device=cuda)
+    ids, gy = torch.tensor([1, 4], device=cuda), torch.randn(2, 8, device=cuda)
+    _, mean, rstd = gna.group_norm_act_forward(x, 2)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: gna.group_norm_act_backward(dual(x), x, mean, rstd, 2),
+                     lambda: gna.group_norm_act_backward(x, dual(x), mean, rstd, 2),
+                     lambda: emb.scaled_embedding(ids, dual(w)),
+                     lambda: emb.scaled_embedding_forward(dual(w), ids),
+                     lambda: emb.scaled_embedding_backward(dual(gy), ids, 5),
+                     lambda: emb.scaled_embedding_backward(gy, ids, 5, grad_weight=dual(w)),
+                     lambda: grad_clip.grad_norm([gy, dual(w)]),
+                     lambda: grad_clip.clip_grads([gy, dual(w)], 1.0),
+                     lambda: grad_clip.clip_grads([gy], 1.0, out=[dual(gy)])):
+            with pytest.raises(NotImplementedError):
+                call()
+
+
+def test_a_function_with_a_derivative_of_its_own_may_call_them(cuda):
+    """Inside a custom Function, where torch takes care of the tangents itself."""
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, w, ids):
+            ctx.ids = ids
+            return emb.scaled_embedding_forward(w, ids, 2.0)
+
+        @staticmethod
+        def jvp(ctx, dw, _):
+            return emb.scaled_embedding_forward(dw, ctx.ids, 2.0)
+
+    w, dw = torch.randn(2, 5, 8, device=cuda)
+    ids = torch.tensor([1, 4, 1], device=cuda)
+    with forward_ad.dual_level():
+        y, dy = forward_ad.unpack_dual(Twice.apply(forward_ad.make_dual(w, dw), ids))
+    assert torch.equal(y, 2 * w[ids]) and torch.equal(dy, 2 * dw[ids])
