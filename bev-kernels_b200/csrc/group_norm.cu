@@ -127,6 +127,11 @@ __device__ __forceinline__ float team_sum(float v, int w) {
   return v;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float exp2_approx(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
@@ -143,7 +148,11 @@ __device__ __forceinline__ float exp2_approx(float t) {
 // Newton step leave (0.05^3)^2 = 1.7e-8: the parameters' gradients are fp32 sums
 // even where the tensors are not.  fp32 tensors get the hardware's reciprocal,
 // and the rounding of -z log2(e) back to first order (at |z| = 10 that is five
-// times the exponential's own error of 2^-22).  The clamps keep infinity out.
+// times the exponential's own error of 2^-22).
+// z is at least kLowest, where d is 2^126.5, the most that the guess's bits stand
+// for.  From d = 2^126 on 1 / d is subnormal, and both ways flush it to zero, so
+// that z sigmoid(z) is zero however far below kLowest z was.
+constexpr float kLowest = -87.68f;
 template <typename T>
 __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -152,7 +161,7 @@ __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
   if constexpr (sizeof(T) == 4) {
     const float2 f = vio::split(z);
     const float lx = fmaf(f.x, -kLog2e, -t.x), ly = fmaf(f.y, -kLog2e, -t.y);
-    float ex = exp2_approx(fminf(t.x, 120.f)), ey = exp2_approx(fminf(t.y, 120.f));
+    float ex = exp2_approx(t.x), ey = exp2_approx(t.y);
     ex = fmaf(ex, lx * kLn2, ex);
     ey = fmaf(ey, ly * kLn2, ey);
     float sx, sy;
@@ -160,7 +169,7 @@ __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sy) : "f"(1.f + ey));
     return vio::two(sx, sy);
   } else {
-    const float ex = exp2_approx(fminf(t.x, 125.f)), ey = exp2_approx(fminf(t.y, 125.f));
+    const float ex = exp2_approx(t.x), ey = exp2_approx(t.y);
     // -d, whose sign bit the guess's constant takes off again
     const vio::Two one = vio::two(1.f);
     const vio::Two minus = vio::fma2(vio::two(ex, ey), vio::two(-1.f), vio::two(-1.f));
@@ -170,8 +179,13 @@ __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
                           __uint_as_float(kGuess - __float_as_uint(m.y)));
     const vio::Two h = vio::fma2(minus, y, one);
     y = vio::fma2(y, vio::fma2(h, h, h), y);
-    return vio::fma2(y, vio::fma2(minus, y, one), y);
+    return vio::fma2_ftz(y, vio::fma2(minus, y, one), y);
   }
+}
+// z, or kLowest where z is below that; a NaN stays
+__device__ __forceinline__ vio::Two from_lowest(vio::Two z) {
+  const float2 f = vio::split(z);
+  return vio::two(max_nan(f.x, kLowest), max_nan(f.y, kLowest));
 }
 template <typename T, int ACT>
 __device__ __forceinline__ vio::Two activate(vio::Two z) {
@@ -179,7 +193,10 @@ __device__ __forceinline__ vio::Two activate(vio::Two z) {
     const float2 f = vio::split(z);
     return vio::two(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);  // NaN stays
   }
-  if constexpr (ACT == BEVK_ACT_SILU) return vio::mul2(z, sigmoid<T>(z));
+  if constexpr (ACT == BEVK_ACT_SILU) {
+    z = from_lowest(z);
+    return vio::mul2(z, sigmoid<T>(z));
+  }
   return z;
 }
 // d act'(z); ReLU's slope is 0 at 0
@@ -190,6 +207,7 @@ __device__ __forceinline__ vio::Two through(vio::Two z, vio::Two d) {
     return vio::two(f.x > 0.f ? g.x : 0.f, f.y > 0.f ? g.y : 0.f);
   }
   if constexpr (ACT == BEVK_ACT_SILU) {
+    z = from_lowest(z);
     const vio::Two s = sigmoid<T>(z);
     const vio::Two rest = vio::fma2(s, vio::two(-1.f), vio::two(1.f));
     return vio::mul2(d, vio::fma2(vio::mul2(z, s), rest, s));

@@ -155,6 +155,12 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
+// the same with subnormal operands and results taken as zero
+__device__ __forceinline__ Two fma2_ftz(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
 __device__ __forceinline__ Two mul2(Two a, Two b) {
   Two r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));

@@ -481,7 +481,7 @@ BEVK_API int bevk_ms_deform_attn_backward(
 enum bevk_activation {
   BEVK_ACT_NONE = 0,
   BEVK_ACT_RELU = 1,
-  BEVK_ACT_SILU = 2 /* z * sigmoid(z) */
+  BEVK_ACT_SILU = 2 /* z * sigmoid(z), 0 at minus infinity */
 };
 
 /*

@@ -344,3 +344,56 @@ def test_refusals(cuda):
         gna.group_norm_act_backward(x[:, :4], x, mean, rstd, 2)
     with pytest.raises(RuntimeError, match="mean and rstd"):
         gna.group_norm_act_backward(x, x, mean.half(), rstd, 2)
+
+
+SILU_Z = [-float("inf"), -3.3e38, -1e36, -1e20, -1000.0, -200.0, -100.0, -89.0, -88.1, -87.8, -87.5,
+          -87.0, -80.0, -40.0, -20.0, -16.5, -10.0, -5.0, -2.5, -1.3, -0.7, -0.1, -1e-3, 0.0]
+SILU_Z = SILU_Z + [-z for z in reversed(SILU_Z[2:])] + [0.5, 3.0]  # 48
+
+
+@pytest.mark.parametrize("c", [48, 47], ids=["vectors", "elements"])
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_silu_at_every_argument(cuda, dt, c):
+    """The activation's argument is the bias alone (weight 0).
+
+    SiLU and its slope have their limits at minus infinity.  The sigmoid s is
+    zero where it would be subnormal, and |z s| is below 88 * 2^-126 there: 2^-119.
+    Else its relative error is that of e^-z (2^-22 of the exponential, |z| units
+    of its rounded argument), which counts 1 - s times, and 6 units of the
+    reciprocal and its step; the slope s (1 + z (1 - s)) has it 1 + |z| times at most.
+    """
+    z = torch.tensor(SILU_Z[:c], device=cuda)
+    g = torch.Generator(cuda).manual_seed(21)
+    x = torch.randn(2, 3, 5, c, generator=g, device=cuda).to(dt).permute(0, 3, 1, 2)
+    gy = torch.randn(2, 3, 5, c, generator=g, device=cuda).to(dt).permute(0, 3, 1, 2)
+    zero = torch.zeros(c, device=cuda)
+    y, mean, rstd = gna.group_norm_act_forward(x, 1, zero, z, EPS, "silu")
+    zd = z.double()
+    s = torch.sigmoid(zd)
+    want = torch.where(zd == -float("inf"), 0.0, zd * s)
+    slope = torch.where(zd.isinf(), (zd > 0).double(), s * (1 + zd * (1 - s)))
+    units = 6 + (4 + zd.abs().clamp_max(200)) * (1 - s)
+    over = want.to(dt).isinf()                                   # +inf, or past the type's range
+    row = y[0, :, 0, 0]
+    assert torch.equal(y, row.view(1, c, 1, 1).expand(y.shape))
+    assert bool((row[over] == float("inf")).all())
+    lim = (units * U32 + UNIT[dt]) * want.abs() + 2.0 ** -119 + (2.0 ** -25 if dt == torch.float16 else 0)
+    assert bool(((row.double() - want).abs() <= lim)[~over].all())
+    gi, gw, gb = gna.group_norm_act_backward(gy, x, mean, rstd, 1, zero, z, "silu")
+    assert not gi.any()
+    total, mag = gy.double().sum((0, 2, 3)), gy.double().abs().sum((0, 2, 3))
+    lim = (units * (1 + zd.abs().clamp_max(200)) * s + 64 * slope.abs()) * U32 * mag + 2.0 ** -119 * mag
+    assert bool(((gb.double() - slope * total).abs() <= lim).all())
+    assert bool(torch.isfinite(gw).all())
+
+
+def test_silu_keeps_nan(cuda):
+    for dt in DTYPES:
+        x = torch.randn(1, 8, 4, 4, device=cuda).to(dt)
+        b = torch.zeros(8, device=cuda)
+        b[3] = float("nan")
+        y, mean, rstd = gna.group_norm_act_forward(x, 8, None, b, EPS, "silu")
+        assert bool(y[:, 3].isnan().all()) and int(y.isnan().sum()) == 16
+        gi, _, gb = gna.group_norm_act_backward(torch.ones_like(x), x, mean, rstd, 8, None, b, "silu")
+        assert bool(gi[:, 3].isnan().all()) and int(gi.isnan().sum()) == 16
+        assert bool(gb[3].isnan()) and int(gb.isnan().sum()) == 1
