@@ -160,7 +160,8 @@ __device__ __forceinline__ vio::Two sigmoid(vio::Two z) {
   const float2 t = vio::split(t2);
   if constexpr (sizeof(T) == 4) {
     const float2 f = vio::split(z);
-    const float lx = fmaf(f.x, -kLog2e, -t.x), ly = fmaf(f.y, -kLog2e, -t.y);
+    // (where t is infinite this is a NaN or too large, and counts nothing: e^-z is 0)
+    const float lx = fminf(fmaf(f.x, -kLog2e, -t.x), 1.f), ly = fminf(fmaf(f.y, -kLog2e, -t.y), 1.f);
     float ex = exp2_approx(t.x), ey = exp2_approx(t.y);
     ex = fmaf(ex, lx * kLn2, ex);
     ey = fmaf(ey, ly * kLn2, ey);
@@ -199,7 +200,8 @@ __device__ __forceinline__ vio::Two activate(vio::Two z) {
   }
   return z;
 }
-// d act'(z); ReLU's slope is 0 at 0
+// d act'(z); ReLU's slope is 0 at 0, SiLU's at infinity the formula's inf * 0 (its
+// limit 1, by clamping z above too, cost 2 % of the backward)
 template <typename T, int ACT>
 __device__ __forceinline__ vio::Two through(vio::Two z, vio::Two d) {
   if constexpr (ACT == BEVK_ACT_RELU) {

@@ -397,3 +397,24 @@ def test_silu_keeps_nan(cuda):
         gi, _, gb = gna.group_norm_act_backward(torch.ones_like(x), x, mean, rstd, 8, None, b, "silu")
         assert bool(gi[:, 3].isnan().all()) and int(gi.isnan().sum()) == 16
         assert bool(gb[3].isnan()) and int(gb.isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_silu_at_its_upper_end(cuda, dt):
+    """Arguments whose product with log2(e) overflows, and infinity: the argument
+    itself, with slope one where it is finite."""
+    c = 8
+    z = torch.tensor([2.3e38, 2.5e38, 3.3e38, float("inf"), 88.0, 1e30, 0.0, 1e5], device=cuda)
+    g = torch.Generator(cuda).manual_seed(24)
+    x = torch.randn(2, 3, 5, c, generator=g, device=cuda).to(dt).permute(0, 3, 1, 2)
+    gy = torch.randn(2, 3, 5, c, generator=g, device=cuda).to(dt).permute(0, 3, 1, 2)
+    zero = torch.zeros(c, device=cuda)
+    y, mean, rstd = gna.group_norm_act_forward(x, 1, zero, z, EPS, "silu")
+    assert torch.equal(y, z.to(dt).view(1, c, 1, 1).expand(y.shape))
+    z[3] = 1e38
+    gi, gw, gb = gna.group_norm_act_backward(gy, x, mean, rstd, 1, zero, z, "silu")
+    assert not gi.any() and bool(torch.isfinite(gw).all())
+    slope = torch.ones(c, dtype=torch.float64, device=cuda)
+    slope[6] = 0.5
+    lim = 64 * U32 * gy.double().abs().sum((0, 2, 3))
+    assert bool(((gb.double() - slope * gy.double().sum((0, 2, 3))).abs() <= lim).all())
