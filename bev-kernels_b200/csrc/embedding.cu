@@ -23,7 +23,7 @@
 // Bound by memory at many tokens (writes alone reach 3.7 to 4 TB/s on this part,
 // reads 5 at these sizes), by the chain of launches and the sort at few.
 // Device time: 65536 rows of 4 KB looked up in 61 us (333 MB, 5.4 TB/s); their
-// gradient added to 10000 fp32 rows in 136 us (430 MB; the sort 20 us of it);
+// gradient added to 10000 fp32 rows in 130 us (430 MB; the sort 20 us of it);
 // 16384 tokens into a dense 50021 x 1024 bf16 table in 41 us (136 MB); 40000
 // tokens of 200 rows of 512 bytes in 19 us, of which the sort is 9; 30 tokens in
 // 12 us, the launches of zeros, sort and sums.
@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "bevk_internal.h"
 #include "bevk_ptx.cuh"
@@ -355,38 +356,29 @@ struct SumParams {
   int accumulate;
 };
 
-// The finished sums of VEC columns, 16 bytes of the output at a time.
+// What the sums of VEC columns are added to, 16 bytes of the output at a time.
+template <typename O, int VEC>
+__device__ __forceinline__ void widen_old(const void *src, float (&old)[VEC]) {
+  constexpr int P = VEC < vio::Full<O>::value ? VEC : vio::Full<O>::value;
+#pragma unroll
+  for (int k = 0; k < VEC; k += P) {
+    float f[P];
+    vio::unpack(vio::load_pack<O, P>(static_cast<const O *>(src) + k), f);
+#pragma unroll
+    for (int e = 0; e < P; ++e) old[k + e] = f[e];
+  }
+}
+template <typename O>
+__device__ __forceinline__ O *place_of(const SumParams &p, unsigned row, int c) {
+  return static_cast<O *>(p.out) + static_cast<int64_t>(row) * p.out_ld + c;
+}
+// The finished sums.  (fp32 atomics in L2 would spare the old values' way here,
+// but they flush subnormals to zero, and round twice.)
 template <typename O, int VEC>
 __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
-                                       const float (&v)[VEC]) {
+                                       const float (&v)[VEC], const float (&old)[VEC]) {
   constexpr int P = VEC < vio::Full<O>::value ? VEC : vio::Full<O>::value;
-  O *dst = static_cast<O *>(p.out) + static_cast<int64_t>(row) * p.out_ld + c;
-  if constexpr (sizeof(O) == 4 && VEC >= 4) {
-    if (p.accumulate) {
-      // nobody else writes these elements: the addition can be left to L2, and
-      // the warp does not wait for the old values
-#pragma unroll
-      for (int k = 0; k < VEC; k += 4)
-        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst + k),
-                     "f"(v[k] * p.scale), "f"(v[k + 1] * p.scale), "f"(v[k + 2] * p.scale),
-                     "f"(v[k + 3] * p.scale)
-                     : "memory");
-      return;
-    }
-  }
-  float old[VEC];
-  if (p.accumulate) {
-#pragma unroll
-    for (int k = 0; k < VEC; k += P) {
-      float f[P];
-      vio::unpack(vio::load_pack<O, P>(dst + k), f);
-#pragma unroll
-      for (int e = 0; e < P; ++e) old[k + e] = f[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) old[e] = 0.f;
-  }
+  O *dst = place_of<O>(p, row, c);
 #pragma unroll
   for (int k = 0; k < VEC; k += P) {
     float f[P];
@@ -395,16 +387,31 @@ __device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
     vio::store<O, P>(dst + k, f);
   }
 }
+template <typename O, int VEC>
+__device__ __forceinline__ void finish(const SumParams &p, unsigned row, int c,
+                                       const float (&v)[VEC]) {
+  float old[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) old[e] = 0.f;
+  if (p.accumulate) widen_old<O, VEC>(place_of<O>(p, row, c), old);
+  finish<O, VEC>(p, row, c, v, old);
+}
 
 constexpr int kSumThreads = 256;
 // Rows on their way per warp: every thread copies its part of them asynchronously
 // into slots of its own in shared memory, so the loop over the tile's tokens is
 // short and a warp waits for its next row only.  (Parts of two bytes, which
 // cannot be copied so, are loaded kBatch rows and kWide columns at a time
-// instead.)  65536 tokens x 2048 columns of bf16 into 10000 fp32 rows: 105 us with
-// 16 rows and 3 CTAs per SM, 104 to 108 with 4 to 24 rows and 8 to 2, and with
-// batches of 16 rows in registers.
-constexpr int kAhead = 16;
+// instead.)  The sums of 65536 tokens x 2048 columns of bf16, their 10000 fp32 rows
+// left to atomics: 105 us with 16 rows and 3 CTAs per SM, 104 to 108 with 4 to 24
+// rows and 8 to 2, and with batches of 16 rows in registers.
+// Where the sums are added to existing rows, the row's old values travel with the
+// last token of its run, and each slot holds both.  65536 x 2048 bf16 added to fp32
+// 130 us with 4 slots, 131 with 8, 142 with 16 (of 8 columns a thread instead of 4:
+// 145 with 8); 65536 x 512 fp32 62, 66, 71; old values loaded where a run ends: 133,
+// 76.
+template <bool ADD>
+constexpr int kAhead = ADD ? 4 : 16;
 constexpr int kBatch = 8, kWide = 4;
 
 // Columns that a warp takes of a tile: 32 of VEC each, or kWide times 32 of two
@@ -412,14 +419,26 @@ constexpr int kBatch = 8, kWide = 4;
 template <typename T, int VEC>
 constexpr int kSliceColumns = 32 * VEC * (sizeof(T) * VEC >= 4 ? 1 : kWide);
 
+// Whether parts of VEC elements of T (and of O, where they are added to those) can
+// be copied asynchronously, and the bytes of shared memory that a thread has for them.
+template <typename T, int VEC>
+constexpr bool kCopied = sizeof(T) * VEC >= 4;
+template <typename T, typename O, int VEC, bool ADD>
+constexpr int kRingBytes =
+    kCopied<T, VEC> ? kAhead<ADD> * static_cast<int>(VEC * (sizeof(T) + (ADD ? sizeof(O) : 0))) : 0;
+
 // One warp per (tile, slice of the columns).
-template <typename T, typename O, int VEC>
+template <typename T, typename O, int VEC, bool ADD>
 __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const SumParams p) {
   constexpr int kBytes = sizeof(T) * VEC;
-  constexpr bool kAsync = kBytes >= 4;
+  constexpr bool kAsync = kCopied<T, VEC>;
   constexpr int W = kAsync ? 1 : kWide;  // a thread's columns are c + 32 w (+ VEC)
+  constexpr int kDepth = kAhead<ADD>;
   constexpr int kSlot = 32 * kBytes;
-  extern __shared__ float4 s_dyn[];  // [warp][kAhead][lane] where copies are asynchronous
+  constexpr int kOldBytes = sizeof(O) * VEC, kOldPart = kOldBytes < 16 ? kOldBytes : 16;
+  // [warp][kDepth][lane] of dy, then of the old values (in parts of 16 bytes at most
+  // [part][lane]), where copies are asynchronous
+  extern __shared__ float4 s_dyn[];
   ptx::grid_launch_dependents();
   ptx::grid_wait_prerequisites();
   const int lane = threadIdx.x & 31;
@@ -437,20 +456,34 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
   const unsigned next = __shfl_down_sync(0xffffffffu, key, 1);
   // bit j: token j is the last of its run within the tile
   const unsigned ends = __ballot_sync(0xffffffffu, lane == 31 || key != next);
+  // bit j: the run lies inside the tile and is finished here (equal ids are together)
+  const unsigned closed = __ballot_sync(0xffffffffu, ((ends >> lane) & 1u) && key != before &&
+                                                         (lane < kTile - 1 || key != after));
   const T *dy = static_cast<const T *>(p.dy) + c;
   const bool col = c < p.dim;
-  char *ring = reinterpret_cast<char *>(s_dyn) + (threadIdx.x >> 5) * kAhead * kSlot + lane * kBytes;
+  char *ring = reinterpret_cast<char *>(s_dyn) + (threadIdx.x >> 5) * kDepth * kSlot + lane * kBytes;
+  char *old_ring = reinterpret_cast<char *>(s_dyn) + kSumThreads / 32 * kDepth * kSlot +
+                   (threadIdx.x >> 5) * kDepth * 32 * kOldBytes + lane * kOldPart;
   const auto row_of = [&](int t) {  // token t's row of dy, for the whole warp
     return dy + static_cast<int64_t>(__shfl_sync(0xffffffffu, pos, t & 31)) * p.dy_ld;
   };
   const auto fetch = [&](int t) {
     const T *src = row_of(t);
-    if (col && t < count) vio::copy_async<kAsync ? kBytes : 4>(ring + t % kAhead * kSlot, src);
+    if (col && t < count) vio::copy_async<kAsync ? kBytes : 4>(ring + t % kDepth * kSlot, src);
+    if constexpr (ADD && kAsync) {
+      const unsigned row = __shfl_sync(0xffffffffu, key, t & 31);
+      if (col && t < count && ((closed >> t) & 1u)) {
+#pragma unroll
+        for (int k = 0; k < kOldBytes; k += kOldPart)
+          vio::copy_async<kOldPart>(old_ring + t % kDepth * 32 * kOldBytes + k * 32,
+                                    reinterpret_cast<const char *>(place_of<O>(p, row, c)) + k);
+      }
+    }
     vio::copy_commit();
   };
   if constexpr (kAsync) {
 #pragma unroll 4
-    for (int t = 0; t < kAhead; ++t) fetch(t);
+    for (int t = 0; t < kDepth; ++t) fetch(t);
   }
   float acc[W][VEC];
   const auto clear = [&] {
@@ -476,8 +509,21 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
         }
       }
     } else {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-      batch[0][0] = vio::load_pack<T, VEC>(ring + t % kAhead * kSlot);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      batch[0][0] = vio::load_pack<T, VEC>(ring + t % kDepth * kSlot);
+    }
+    float old[VEC];
+    if constexpr (ADD && kAsync) {
+      if ((closed >> t) & 1u) {
+#pragma unroll
+        for (int k = 0; k < kOldBytes; k += kOldPart) {
+          constexpr int P = kOldPart / sizeof(O);
+          float f[P];
+          vio::unpack(vio::load_pack<O, P>(old_ring + t % kDepth * 32 * kOldBytes + k * 32), f);
+#pragma unroll
+          for (int e = 0; e < P; ++e) old[k / static_cast<int>(sizeof(O)) + e] = f[e];
+        }
+      }
     }
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -490,11 +536,11 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
 #pragma unroll
       for (int j = 0; j + 1 < (kAsync ? 1 : kBatch); ++j) batch[j][w] = batch[j + 1][w];
     }
-    if constexpr (kAsync) fetch(t + kAhead);
+    if constexpr (kAsync) fetch(t + kDepth);
     if (!((ends >> t) & 1u)) continue;
     const unsigned row = __shfl_sync(0xffffffffu, key, t);
     const bool goes_on = t == kTile - 1 && after == row;
-    const bool open = (begin == 0 && before == row) || goes_on;
+    const bool open = !((closed >> t) & 1u);
     if (goes_on && !(begin == 0 && before == row) && c == 0) {
       // where the run still is if it has more pieces; the lists' order changes nothing
       const int64_t far = first + int64_t(kShort) * kTile;
@@ -517,6 +563,8 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(const Sum
 #pragma unroll
           for (int k = 0; k < VEC; ++k) __stcg(dst + k, acc[w][k]);
         }
+      } else if constexpr (ADD && kAsync) {
+        finish<O, VEC>(p, row, cw, acc[w], old);
       } else {
         finish<O, VEC>(p, row, cw, acc[w]);
       }
@@ -752,7 +800,7 @@ int sort_any(const SortParams &p, cudaStream_t stream) {
   return sort_ids<Id, 0>(p, cluster, stream);
 }
 
-template <typename T, typename O, int VEC>
+template <typename T, typename O, int VEC, bool ADD>
 int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
   SumParams p = p0;
   p.slices = (p.dim + kSliceColumns<T, VEC> - 1) / kSliceColumns<T, VEC>;
@@ -760,20 +808,20 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
   const int64_t grid = (warps + per - 1) / per;
   if (grid >= (int64_t(1) << 31))
     return fail(BEVK_ERR_INDEX_OVERFLOW, "embedding_backward: too many tokens and columns");
-  const size_t smem = sizeof(T) * VEC >= 4 ? sizeof(T) * VEC * kAhead * kSumThreads : 0;
+  const size_t smem = static_cast<size_t>(kRingBytes<T, O, VEC, ADD>) * kSumThreads;
   if (smem > 0) {
     static thread_local int seen_device = -1;
     const int dev = current_device();
     if (dev < 0) return fail(BEVK_ERR_CUDA, "embedding_backward: no device");
     if (seen_device != dev) {
-      const cudaError_t e = cudaFuncSetAttribute(embedding_sum_kernel<T, O, VEC>,
+      const cudaError_t e = cudaFuncSetAttribute(embedding_sum_kernel<T, O, VEC, ADD>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(smem));
       if (e != cudaSuccess) return launched(e, "embedding_sum_kernel");
       seen_device = dev;
     }
   }
-  const int st = launched(launch_dependent(embedding_sum_kernel<T, O, VEC>,
+  const int st = launched(launch_dependent(embedding_sum_kernel<T, O, VEC, ADD>,
                                            dim3(static_cast<unsigned>(grid)), dim3(kSumThreads),
                                            smem, stream, p),
                           "embedding_sum_kernel");
@@ -788,17 +836,23 @@ int sum(const SumParams &p0, int64_t tiles, cudaStream_t stream) {
                   "embedding_join_kernel");
 }
 
-// The widest part of a row, up to 16 bytes, that every row's start and length are
-// a multiple of on the side of dy, and its columns on the side of the table.
-template <typename T, typename O, int VEC = vio::Full<T>::value>
+// The widest part of a row, up to 16 bytes of dy (of the wider side where both are
+// copied), that every row's start and length are a multiple of on the side of dy, and
+// its columns on the side of the table.
+template <typename T, typename O, bool ADD, int VEC = vio::Full<std::conditional_t<ADD, O, T>>::value>
 int sum_any(const SumParams &p, int64_t tiles, cudaStream_t stream) {
   constexpr size_t kOut = std::min<size_t>(16, VEC * sizeof(O));
   const bool fits = p.dim % VEC == 0 && p.dy_ld % VEC == 0 && aligned(p.dy, VEC * sizeof(T)) &&
                     p.out_ld * sizeof(O) % kOut == 0 && aligned(p.out, kOut);
   if constexpr (VEC > 1) {
-    if (!fits) return sum_any<T, O, VEC / 2>(p, tiles, stream);
+    if (!fits) return sum_any<T, O, ADD, VEC / 2>(p, tiles, stream);
   }
-  return sum<T, O, VEC>(p, tiles, stream);
+  return sum<T, O, VEC, ADD>(p, tiles, stream);
+}
+template <typename T, typename O>
+int sum_any(const SumParams &p, int64_t tiles, cudaStream_t stream) {
+  return p.accumulate ? sum_any<T, O, true>(p, tiles, stream)
+                      : sum_any<T, O, false>(p, tiles, stream);
 }
 
 }  // namespace

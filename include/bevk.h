@@ -559,7 +559,8 @@ typedef struct bevk_embedding_backward_args {
   int grad_table_dtype;    /* grad_output's dtype or fp32                      */
   int accumulate;          /* 0: every element of grad_table is written (rows
                               no id names get zeros); 1: the sums are added to
-                              the rows that ids name, others are not touched   */
+                              the rows that ids name (old + scale * sum,
+                              rounded once), others are not touched            */
 } bevk_embedding_backward_args;
 
 /* Scratch bytes of the backward; 256-byte aligned, needs no initialisation. */

@@ -289,3 +289,54 @@ def test_dense_gradient_into_a_wider_buffer(cuda):
         want = torch.zeros(50, dim, device=cuda)
         want[3], want[49] = 2, 1
         assert torch.equal(rows[:, :dim], want)
+
+
+def abi_backward(gy, ids, grad_table, rows, dim, ld, accumulate=0, at=0, scale=1.0):
+    """The C ABI with grad_table's first element `at` elements into the buffer."""
+    import ctypes
+
+    from bevk import cabi
+    L, code = cabi.lib(), {torch.float32: cabi.DTYPE_F32, torch.float16: cabi.DTYPE_F16,
+                           torch.bfloat16: cabi.DTYPE_BF16}
+    a = cabi.EmbeddingBackwardArgs()
+    a.num_ids, a.num_rows, a.dim, a.ids_are_64bit = ids.numel(), rows, dim, 1
+    a.grad_output_ld, a.grad_table_ld, a.padding_idx, a.scale = dim, ld, -1, scale
+    a.grad_output_dtype, a.grad_table_dtype = code[gy.dtype], code[grad_table.dtype]
+    a.accumulate = accumulate
+    n = L.bevk_embedding_backward_workspace_bytes(ctypes.byref(a))
+    ws = torch.empty(n, dtype=torch.uint8, device=gy.device)
+    cabi.check(L.bevk_embedding_backward(
+        ctypes.byref(a), gy.data_ptr(), ids.data_ptr(),
+        grad_table.data_ptr() + at * grad_table.element_size(), ws.data_ptr(), n,
+        torch.cuda.current_stream().cuda_stream), "embedding_backward")
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_adding_keeps_subnormals_and_rounds_alike_at_any_alignment(cuda, dt):
+    """old + scale * (the row's sum), rounded once: whichever width the rows are
+    taken in, and below the smallest normal number too."""
+    g = torch.Generator(cuda).manual_seed(11)
+    rows, dim, n = 60, 32, 500
+    ids = ids_of("skewed", n, rows, cuda)
+    gy = torch.randn(n, dim, generator=g, device=cuda).to(dt)
+    old = torch.randn(rows, dim, generator=g, device=cuda)
+    got = []
+    for ld, at in ((dim, 0), (dim + 1, 0), (dim, 1), (dim + 4, 4)):
+        buf = torch.zeros(rows * ld + at, device=cuda)
+        view = buf[at:].view(rows, ld)[:, :dim]
+        view.copy_(old)
+        abi_backward(gy, ids, buf, rows, dim, ld, accumulate=1, at=at, scale=1.7)
+        got.append(view.clone())
+    assert all(torch.equal(t, got[0]) for t in got[1:])
+    # a named row's subnormal elements, and sums that are subnormal or become so
+    main = torch.full((4, dim), 3e-40, device=cuda)
+    gy = torch.zeros(3, dim, device=cuda)
+    gy[1] = 5e-41
+    gy[2] = 1.0
+    kept = main.clone()
+    emb.scaled_embedding_backward(gy, torch.tensor([0, 1, 2], device=cuda), 4, 2.0 ** -130,
+                                  grad_weight=main)
+    want = kept.double()
+    want[1] += 2.0 ** -130 * gy[1].double()
+    want[2] += 2.0 ** -130
+    assert torch.equal(main, want.float())
