@@ -13,7 +13,8 @@
 //
 // The tensors are cut into tiles of one size (a tensor's last one is shorter)
 // and every CTA takes a contiguous run of tiles.  Squares are summed in fp32
-// within a tile and thread, and those sums in fp64 in a fixed order.
+// within a tile and thread (in fp64 where they leave its range), and those sums in
+// fp64 in a fixed order.
 //
 // Bound by memory: 68 M bf16 elements clipped into fp32 take 97 us on the device
 // (136 MB read twice, 272 MB written: 5.6 TB/s), 28 us of it the norm, whose rate
@@ -93,12 +94,43 @@ __device__ __forceinline__ int head_of(const T *p, int n, int bytes) {
   return min(n, off ? (bytes - off) / static_cast<int>(sizeof(T)) : 0);
 }
 
+// A thread's squares of a tile in fp64, for those that leave fp32's range: the same
+// elements as below.
+template <typename T>
+__device__ __noinline__ double wide_squares(const T *p, int n) {
+  constexpr int V = vio::Full<T>::value;
+  const int tid = threadIdx.x, head = head_of(p, n, 16);
+  double sum = 0.0;
+  const auto take = [&](T e) {
+    const double v = vio::widen(e);
+    sum = fma(v, v, sum);
+  };
+  if (tid < head) take(p[tid]);
+  const T *body = p + head;
+  const int vecs = (n - head) / V;
+  for (int i = tid; i < vecs; i += kThreads)
+    for (int e = 0; e < V; ++e) take(body[i * V + e]);
+  if (tid < n - head - vecs * V) take(body[vecs * V + tid]);
+  return sum;
+}
+
+// Squares are summed in fp32, which holds them to its precision while the result
+// is not below 2^-100 (what is lost of subnormal squares is 2^-144 at most) and
+// does not overflow; else, except where all elements are zero, once more in fp64.
+constexpr float kLeastSquares = 0x1p-100f, kMostSquares = 0x1.fffffep127f;
+
 template <typename T, bool INF>
-__device__ __forceinline__ float norm_tile(const T *p, int n) {
+__device__ __forceinline__ double norm_tile(const T *p, int n) {
   constexpr int V = vio::Full<T>::value, B = kBatch;
   Sum<INF> s;
+  unsigned bits = 0;  // whether any element is not zero
   const int tid = threadIdx.x, head = head_of(p, n, 16);
-  if (tid < head) s.take(0, vio::widen(p[tid]));
+  const auto take_one = [&](int k, T e) {
+    const float v = vio::widen(e);
+    s.take(k, v);
+    bits |= __float_as_uint(fabsf(v));
+  };
+  if (tid < head) take_one(0, p[tid]);
   const T *body = p + head;
   const int vecs = (n - head) / V;
   const auto take = [&](const vio::Pack<T, V> &q) {
@@ -106,6 +138,7 @@ __device__ __forceinline__ float norm_tile(const T *p, int n) {
     vio::unpack(q, f);
 #pragma unroll
     for (int e = 0; e < V; ++e) s.take(e, f[e]);
+    if (!INF) bits |= (q.w[0] | q.w[1] | q.w[2] | q.w[3]) & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu);
   };
   int i = tid;
   for (; i + (B - 1) * kThreads < vecs; i += B * kThreads) {
@@ -117,8 +150,10 @@ __device__ __forceinline__ float norm_tile(const T *p, int n) {
   }
   for (; i < vecs; i += kThreads) take(vio::load_pack<T, V>(body + i * V));
   const int tail = n - head - vecs * V;
-  if (tid < tail) s.take(1, vio::widen(body[vecs * V + tid]));
-  return s.value();
+  if (tid < tail) take_one(1, body[vecs * V + tid]);
+  const float v = s.value();
+  if (!INF && ((v < kLeastSquares && bits != 0) || !(v <= kMostSquares))) return wide_squares(p, n);
+  return v;
 }
 
 // Scales one tile.  A thread takes as many elements at a time as make 16 bytes
@@ -193,7 +228,7 @@ __device__ double cta_reduce(double v, bool inf_norm, double *s_part) {
 }
 
 template <typename T>
-__device__ __forceinline__ float norm_any(const void *p, int64_t at, int n, bool inf_norm) {
+__device__ __forceinline__ double norm_any(const void *p, int64_t at, int n, bool inf_norm) {
   const T *q = static_cast<const T *>(p) + at;
   return inf_norm ? norm_tile<T, true>(q, n) : norm_tile<T, false>(q, n);
 }
@@ -219,13 +254,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       while (t >= p.first_tile[k + 1]) ++k;
       const int64_t at = static_cast<int64_t>(t - p.first_tile[k]) * p.tile;
       const int n = static_cast<int>(min(static_cast<int64_t>(p.tile), p.numel[k] - at));
-      float v;
+      double v;
       switch (p.types[k] & 3) {
         case BEVK_DTYPE_F16: v = norm_any<__half>(p.in[k], at, n, inf_norm); break;
         case BEVK_DTYPE_BF16: v = norm_any<__nv_bfloat16>(p.in[k], at, n, inf_norm); break;
         default: v = norm_any<float>(p.in[k], at, n, inf_norm);
       }
-      sum = inf_norm ? max_nan(sum, static_cast<double>(v)) : sum + v;
+      sum = inf_norm ? max_nan(sum, v) : sum + v;
     }
     sum = cta_reduce(sum, inf_norm, s_part);
     if (threadIdx.x == 0) __stcg(p.partial + blockIdx.x, sum);

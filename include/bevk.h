@@ -594,8 +594,9 @@ BEVK_API size_t bevk_grad_clip_workspace_bytes(int num_tensors);
  *   out = c * g (rounded once),  norm_out[0] = norm (fp32, device memory).
  * scale = 0 only takes the norm (out is ignored).  A NaN in any gradient makes
  * the norm NaN and with it every output; an infinite norm gives c = 0.  In
- * place, c = 1 writes nothing.  Squares are fp32 and their sums fp64: a
- * gradient above 1.8e19 makes the norm infinite.  Outputs must not overlap one another, nor a
+ * place, c = 1 writes nothing.  Only the norm itself has to fit fp32: squares and
+ * sums are fp32 within a thread's share of a tile where that holds them, else fp64,
+ * and fp64 beyond.  Outputs must not overlap one another, nor a
  * gradient other than their own.  tensors is host memory, read before the
  * call returns.  Equal inputs give equal bits (no floating-point atomics).
  */

@@ -235,3 +235,36 @@ def test_c_abi_checks_before_any_launch(cuda):
     t = (cabi.GradTensor * 1)()
     t[0].grad, t[0].out, t[0].numel = 6, 6, 4                    # not aligned to fp32
     assert L.bevk_grad_clip(t, 1, 0, 1.0, 1e-6, 1, 16, 16, 1 << 20, None) == cabi.ERR_MISALIGNED
+
+
+@pytest.mark.parametrize("n", [37, 5000, 10_000_000])
+@pytest.mark.parametrize("size", [1e37, 5e18, 1e10, 1e-10, 1e-19, 1e-24, 1e-30, 1e-38])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_norms_over_the_range_of_fp32(cuda, dt, size, n):
+    """Only the norm itself has to fit fp32, not the squares or their sums."""
+    if size * n ** 0.5 > 1e38:
+        n = 50
+    g = torch.Generator(cuda).manual_seed(8)
+    # the same magnitudes in every thread's share, within a factor of two
+    flat = ((0.5 + torch.rand(n, generator=g, device=cuda)) * size).to(dt)
+    flat *= torch.where(torch.rand(n, generator=g, device=cuda) < 0.5, -1.0, 1.0).to(dt)
+    grads = [flat[:1], flat[1:4], flat[4:]]
+    before = [t.clone() for t in grads]
+    ref = want_norm(grads)
+    assert abs(float(grad_clip.grad_norm(grads)) - ref) <= 16 * U32 * ref + 2.0 ** -149
+    check(grad_clip.clip_grads(grads, 0.5 * ref), grads, before, 0.5 * ref)
+
+
+def test_small_and_large_among_others(cuda):
+    g = torch.full((10_000_000,), 1e-30, device=cuda)
+    zeros = torch.zeros(1_000_000, device=cuda)
+    zeros[::2] = -0.0
+    for at, v in ((5, 1e-3), (9_999_999, -1e25), (4_000_001, 1e-20)):
+        t = g.clone()
+        t[at] = v
+        ref = want_norm([t])
+        assert abs(float(grad_clip.grad_norm([zeros, t])) - ref) <= 16 * U32 * ref
+    assert float(grad_clip.grad_norm([zeros])) == 0.0
+    # a norm past fp32's range is infinite and scales by zero
+    t = torch.full((2,), 3e38, device=cuda)
+    assert float(grad_clip.clip_grads([t], 1.0)) == math.inf and not t.any()
