@@ -8,9 +8,16 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <string>
+
 #include "bevk.h"
 
 namespace bevk_ext {
+
+// Integers go into messages as text: streaming one from an extension crashes
+// where the interpreter has loaded another C++ runtime library than the one
+// that the extension was built with.
+inline std::string str(int64_t v) { return std::to_string(v); }
 
 inline int dtype_of(const at::Tensor &t) {
   switch (t.scalar_type()) {

@@ -30,8 +30,8 @@ void col_common(const Tensor &data_im, const Tensor &data_offset, const Tensor &
               "bevk: im2col tensors must share data_im's dtype");
   const int64_t T = int64_t(kernel_h) * kernel_w;
   const int64_t need = int64_t(channels) * T * batch_size * height_col * width_col;
-  TORCH_CHECK(data_col.numel() == need, "bevk: data_col has ", data_col.numel(),
-              " elements, expected ", need);
+  TORCH_CHECK(data_col.numel() == need, "bevk: data_col has ", str(data_col.numel()),
+              " elements, expected ", str(need));
   const c10::cuda::CUDAGuard guard(data_im.device());
   int st;
   if (layout == 0) {
@@ -275,7 +275,7 @@ void dcn_forward(const Tensor &input, const Tensor &offset, const Tensor &mask,
   int ho = 0, wo = 0;
   check_status(bevk_dcn_output_size(&p, &ho, &wo), "dcn_forward");
   TORCH_CHECK(output.size(0) == p.batch && output.size(2) == ho && output.size(3) == wo,
-              "bevk: output must be [", p.batch, ", Cout, ", ho, ", ", wo, "]");
+              "bevk: output must be [", str(p.batch), ", Cout, ", str(ho), ", ", str(wo), "]");
   TORCH_CHECK(offset.size(0) == p.batch && offset.size(1) == 2 * deform_groups * kernel_h * kernel_w &&
                   offset.size(2) == ho && offset.size(3) == wo,
               "bevk: offset must be [B, 2*dg*kH*kW, Ho, Wo]");
@@ -346,8 +346,8 @@ void col2im_common(const Tensor &dcol, const Tensor *data_im, const Tensor &offs
   const int T = kernel_h * kernel_w;
   const int64_t M = static_cast<int64_t>(batch) * height_col * width_col;
   TORCH_CHECK(dcol.numel() == static_cast<int64_t>(channels) * T * M, "bevk: ", what,
-              ": the column gradient has ", dcol.numel(), " elements, expected ",
-              static_cast<int64_t>(channels) * T * M);
+              ": the column gradient has ", str(dcol.numel()), " elements, expected ",
+              str(static_cast<int64_t>(channels) * T * M));
   const at::ScalarType xt = offset.scalar_type();
   TORCH_CHECK(mask.scalar_type() == xt && (!data_im || data_im->scalar_type() == xt),
               "bevk: ", what, ": data_im / offset / mask must share a dtype");

@@ -17,11 +17,6 @@ namespace {
 
 using OptTensor = std::optional<Tensor>;
 
-// Integers go into messages as text: streaming one from an extension crashes
-// where the interpreter has loaded another C++ runtime library than the one
-// that the extension was built with.
-std::string str(int64_t v) { return std::to_string(v); }
-
 // Counts a write through a tensor's pointer, as torch's own operators count theirs:
 // a graph that saved the tensor before then refuses the new values.  (Inference
 // tensors are not counted.)
