@@ -4,8 +4,8 @@ Camera features pass a deformable convolution and a group norm with SiLU; a
 grid of queries, looked up with learned row and column positions, samples them
 with deformable attention; a group norm with ReLU and a 1x1 convolution give a
 map.  After the backward pass the gradients are clipped to a global norm and
-the weights take a step.  Everything stays channels-last; nothing in the step
-synchronises except the loss that is printed.
+the weights take a step.  Everything stays channels-last, and after the first
+step nothing in a step waits for the device.
 
     python examples/bev_train_step.py [--steps 20] [--dtype bf16]
 """
@@ -46,6 +46,15 @@ class BevHead(nn.Module):
         r, c = torch.meshgrid(torch.arange(rows), torch.arange(cols), indexing="ij")
         self.register_buffer("row_ids", r.reshape(-1))
         self.register_buffer("col_ids", c.reshape(-1))
+        self._levels = {}  # (h, w, device): a copy from the host would wait in every step
+
+    def levels(self, h: int, w: int, device):
+        """The attention's shapes and level starts of one [h, w] level."""
+        key = (h, w, device)
+        if key not in self._levels:
+            self._levels[key] = (torch.tensor([[h, w]], device=device),
+                                 torch.zeros(1, dtype=torch.int64, device=device))
+        return self._levels[key]
 
     def forward(self, feats: torch.Tensor) -> torch.Tensor:
         n, c, h, w = feats.shape
@@ -58,8 +67,7 @@ class BevHead(nn.Module):
             self.offsets(query)).view(q, self.heads, 1, self.points, 2)
         att = self.weights(query).view(q, self.heads, self.points).softmax(-1).view(
             q, self.heads, 1, self.points)
-        shapes = torch.tensor([[h, w]], device=feats.device)
-        start = torch.zeros(1, dtype=torch.int64, device=feats.device)
+        shapes, start = self.levels(h, w, feats.device)
         seen = multi_scale_deformable_attn(
             value.contiguous(), shapes, start, loc.expand(n, q, self.heads, 1, self.points, 2).contiguous(),
             att.expand(n, q, self.heads, 1, self.points).contiguous(), 64)

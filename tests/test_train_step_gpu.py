@@ -65,3 +65,28 @@ def test_every_parameter_gets_the_gradient_of_the_plain_operators(cuda):
     for n in own:
         # chains of a few hundred fp32 roundings through two norms and the attention
         assert float((own[n] - plain[n]).norm()) <= 1e-4 * float(plain[n].norm()) + 1e-6, n
+
+
+def test_the_step_does_not_wait_for_the_device(cuda):
+    """Forward, backward, clipping and the weights' step are only queued."""
+    import bev_train_step
+    from torch import nn
+    model = bev_train_step.BevHead(64, 12, 10, 3).to(cuda)
+    feats = torch.randn(2, 64, 9, 11, device=cuda).contiguous(memory_format=torch.channels_last)
+    target = torch.randint(0, 3, (1, 12, 10), device=cuda)
+    opt = torch.optim.SGD(model.parameters(), lr=0.05, momentum=0.9)
+
+    def step():
+        loss = nn.functional.cross_entropy(model(feats).float()[None], target)
+        opt.zero_grad(set_to_none=True)
+        loss.backward()
+        bev_train_step.clip_grad_norm_(model.parameters(), 1.0)
+        opt.step()
+
+    step()                                                       # what is set up once
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        step()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
