@@ -340,3 +340,37 @@ def test_adding_keeps_subnormals_and_rounds_alike_at_any_alignment(cuda, dt):
     want[1] += 2.0 ** -130 * gy[1].double()
     want[2] += 2.0 ** -130
     assert torch.equal(main, want.float())
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,dim", [(5, 8), (40, 33), (900, 64), (5000, 136), (60000, 24)])
+def test_zeros_stay_inside_the_table(cuda, rows, dim, dt):
+    """Tables below and above the size whose zeros get a kernel of their own, at
+    any element offset, back to back and with gaps between the rows."""
+    gy = torch.ones(2, dim, device=cuda, dtype=dt)
+    ids = torch.tensor([rows - 1, 1], device=cuda)
+    for ld in (dim, dim + 8, dim + 3):
+        for at in (0, 1, 3, 7):
+            buf = torch.full((at + rows * ld + 40,), 7.0, device=cuda, dtype=dt)
+            abi_backward(gy, ids, buf, rows, dim, ld, at=at)
+            table = buf[at:at + rows * ld].view(rows, ld)
+            assert bool((buf[:at] == 7).all()) and bool((buf[at + rows * ld:] == 7).all())
+            assert bool((table[:, dim:] == 7).all())
+            want = torch.zeros(rows, dim, device=cuda, dtype=dt)
+            want[rows - 1] = want[1] = 1
+            assert torch.equal(table[:, :dim], want)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("n,rows,dim,kind", [(1000, 255, 40, "skewed"), (5000, 3000, 33, "uniform"),
+                                             (30000, 7, 520, "one"), (37, 50, 6, "uniform")])
+def test_added_to_a_16_bit_gradient(cuda, n, rows, dim, kind, dt):
+    g = torch.Generator(cuda).manual_seed(12)
+    ids = ids_of(kind, n, rows, cuda)
+    gy = torch.randn(n, dim, generator=g, device=cuda).to(dt)
+    main = torch.randn(rows, dim, generator=g, device=cuda).to(dt)
+    old = main.clone()
+    emb.scaled_embedding_backward(gy, ids, rows, 0.5, grad_weight=main)
+    want = expected(gy, ids, rows, 0.5, None, old)
+    check(main, want)
+    assert torch.equal(main[want[2] == 0], old[want[2] == 0])
