@@ -90,3 +90,28 @@ def test_the_step_does_not_wait_for_the_device(cuda):
         step()
     finally:
         torch.cuda.set_sync_debug_mode("default")
+
+
+def test_meetings_of_two_streams_do_not_mix(cuda):
+    """Launches whose CTAs meet, on two streams at once: each starts when all of
+    its CTAs fit, and results are those of the calls one after the other."""
+    import grad_clip
+    import group_norm_act as gna
+    g = torch.Generator(cuda).manual_seed(2)
+    x = torch.randn(4, 60, 50, 128, generator=g, device=cuda).half().permute(0, 3, 1, 2)
+    _, mean, rstd = gna.group_norm_act_forward(x, 8, act="silu")
+    grads = [torch.randn(k, generator=g, device=cuda) for k in (5, 300_000, 77, 1_000_000)]
+    out = [torch.empty_like(t) for t in grads]
+    want = gna.group_norm_act_backward(x, x, mean, rstd, 8, act="silu")[0]
+    norm = grad_clip.clip_grads(grads, 1.0, out=out).clone()
+    clipped = [o.clone() for o in out]
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(one):
+            got = gna.group_norm_act_backward(x, x, mean, rstd, 8, act="silu")[0]
+        with torch.cuda.stream(two):
+            again = grad_clip.clip_grads(grads, 1.0, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(again, norm)
+    assert all(torch.equal(a, b) for a, b in zip(out, clipped))
