@@ -145,10 +145,11 @@ __device__ __forceinline__ float exp2_approx(float t) {
 // subtraction from d's bits gives: y d = (1 + m)(2 - m - s) / 2 with the shift
 // s = 5 - sqrt(24) that makes the error the same at m = 0 and in the middle
 // (s / 2 = 5 %).  A third-order step, y (1 + h + h^2) with h = 1 - y d, and a
-// Newton step leave (0.05^3)^2 = 1.7e-8: the parameters' gradients are fp32 sums
-// even where the tensors are not.  fp32 tensors get the hardware's reciprocal,
-// and the rounding of -z log2(e) back to first order (at |z| = 10 that is five
-// times the exponential's own error of 2^-22).
+// Newton step leave (0.05^3)^2 = 1.7e-8, less than the two units of 2^-24 that the
+// roundings add: the parameters' gradients are fp32 sums even where the tensors are
+// not.  fp32 tensors get the hardware's reciprocal, and the rounding of -z log2(e)
+// back to first order (at |z| = 10 that is five times the exponential's own error of
+// 2^-22).
 // z is at least kLowest, where d is 2^126.5, the most that the guess's bits stand
 // for.  From d = 2^126 on 1 / d is subnormal, and both ways flush it to zero, so
 // that z sigmoid(z) is zero however far below kLowest z was.

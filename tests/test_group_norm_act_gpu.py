@@ -418,3 +418,47 @@ def test_silu_at_its_upper_end(cuda, dt):
     slope[6] = 0.5
     lim = 64 * U32 * gy.double().abs().sum((0, 2, 3))
     assert bool(((gb.double() - slope * gy.double().sum((0, 2, 3))).abs() <= lim).all())
+
+
+def test_the_16_bit_sigmoid_is_good_to_a_few_units(cuda):
+    """grad_bias is an fp32 sum also for 16-bit tensors; with one nonzero
+    gradient a channel it is the slope itself.  Error of the slope as in
+    test_silu_at_every_argument; near zero that is 9 units of 2^-24."""
+    c = 4096
+    z = torch.linspace(-30, 30, c, device=cuda)
+    for dt in (torch.float16, torch.bfloat16):
+        x = torch.randn(1, c, 1, 2, generator=torch.Generator(cuda).manual_seed(22), device=cuda).to(dt)
+        gy = torch.zeros_like(x)
+        gy[..., 0] = 1
+        zero = torch.zeros(c, device=cuda)
+        _, mean, rstd = gna.group_norm_act_forward(x, 1, zero, z, EPS, "silu")
+        _, _, gb = gna.group_norm_act_backward(gy, x, mean, rstd, 1, zero, z, "silu")
+        zd = z.double()
+        s = torch.sigmoid(zd)
+        slope = s * (1 + zd * (1 - s))
+        units = 6 + (4 + zd.abs()) * (1 - s)
+        lim = (units * (1 + zd.abs()) * s + 3 * slope.abs()) * U32
+        assert bool(((gb.double() - slope).abs() <= lim).all())
+
+
+def test_offsets_past_31_bits(cuda):
+    """2.2e9 elements in two images of a repeated block, whose statistics are the
+    block's.  A thread's fp32 chains are some 15000 terms long here; rounding
+    errors add up like a random walk, to about sqrt(15000) units: 512 allowed."""
+    n, c, hw, part = 2, 64, 17_000_000, 1000
+    g = torch.Generator(cuda).manual_seed(23)
+    block = torch.randn(n, part, c, generator=g, device=cuda)
+    block = (block + torch.tensor([0.0, 2.0], device=cuda).view(n, 1, 1)).bfloat16()
+    x = torch.empty(n, hw, c, dtype=torch.bfloat16, device=cuda)
+    x.view(n, hw // part, part, c).copy_(block[:, None].expand(n, hw // part, part, c))
+    x, small = x.permute(0, 2, 1), block.permute(0, 2, 1)
+    y, mean, rstd = gna.group_norm_act_forward(x, 8, act="silu")
+    ref = reference(small, small, None, None, 8, "silu")
+    assert bool(((mean.double() - ref["mean"]).abs() <= 512 * U32 * (1 + ref["mean"].abs())).all())
+    assert bool(((rstd.double() / ref["rstd"] - 1).abs() <= 512 * U32).all())
+    limit = UNIT[torch.bfloat16] + 512 * U32 * (1 + ref["ratio"])
+    gi, _, _ = gna.group_norm_act_backward(x, x, mean, rstd, 8, act="silu")
+    for t, want in ((y, ref["y"]), (gi, ref["dx"])):
+        assert rel_l2(t[:, :, -part:], want) <= limit
+        parts = t.permute(0, 2, 1).reshape(n, hw // part, part, c)
+        assert bool((parts == parts[:, :1]).all())               # every repetition alike
