@@ -2,6 +2,7 @@
 // (group norm with activation on channels-last tensors, embedding lookup with
 // scaling, the global gradient norm and clipping) over the C ABI.
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <torch/csrc/autograd/forward_grad.h>
 
 #include <optional>
 #include <string>
@@ -27,12 +28,23 @@ void count_write(const Tensor &t) {
 // The operators have no forward-mode derivative.  A tangent is refused, as torch
 // refuses it for a Function without one: the result would have none, which reads
 // as a derivative of zero.  (In the forward of a custom Function forward mode is
-// off: what is called there has its derivative from the Function.)
-void check_no_tangent(const Tensor &t, const char *name) {
-  TORCH_CHECK_NOT_IMPLEMENTED(
-      !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
-      "bevk: ", name, " has a forward-mode tangent; this operator has no forward-mode derivative");
+// off: what is called there has its derivative from the Function.)  Tensors can
+// have tangents only within a dual level, which is asked for once a call.
+bool tangents_possible() {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+         torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
 }
+void check_no_tangent(const Tensor &t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(),
+                              "bevk: a tensor has a forward-mode tangent; this operator has no "
+                              "forward-mode derivative");
+}
+void check_no_tangents(std::initializer_list<const Tensor *> tensors) {
+  if (!tangents_possible()) return;
+  for (const Tensor *t : tensors)
+    if (t) check_no_tangent(*t);
+}
+const Tensor *opt_ptr(const OptTensor &t) { return t ? &*t : nullptr; }
 
 // ------------------------------------------------------- group norm + act
 
@@ -87,7 +99,7 @@ bevk_group_norm_problem gn_problem(const Tensor &input, int64_t num_groups,
                                    const OptTensor &weight, const OptTensor &bias, double eps,
                                    int64_t act) {
   check_cuda(input, "input");
-  check_no_tangent(input, "input");
+  check_no_tangents({&input, opt_ptr(weight), opt_ptr(bias)});
   TORCH_CHECK(input.dim() >= 2, "bevk: input must be [N, C, *spatial]");
   TORCH_CHECK(num_groups > 0 && input.size(1) > 0 && input.size(1) % num_groups == 0,
               "bevk: num_groups=", str(num_groups), " must divide the channels (",
@@ -101,7 +113,6 @@ bevk_group_norm_problem gn_problem(const Tensor &input, int64_t num_groups,
   for (const OptTensor *t : {&weight, &bias}) {
     if (!*t) continue;
     check_same_device(input, **t, "weight / bias");
-    check_no_tangent(**t, "weight / bias");
     TORCH_CHECK((*t)->dim() == 1 && (*t)->size(0) == input.size(1) && (*t)->is_contiguous(),
                 "bevk: weight and bias must be contiguous [C]");
     const int dt = dtype_of(**t);
@@ -156,10 +167,9 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(
     int64_t num_groups, const OptTensor &weight, const OptTensor &bias, int64_t act,
     bool need_input, bool need_weight, bool need_bias) {
   bevk_group_norm_problem p = gn_problem(input_, num_groups, weight, bias, 0.0, act);
-  for (const Tensor *t : {&grad_output_, &mean, &rstd}) {
+  for (const Tensor *t : {&grad_output_, &mean, &rstd})
     check_same_device(input_, *t, "group norm tensor");
-    check_no_tangent(*t, "group norm tensor");
-  }
+  check_no_tangents({&grad_output_, &mean, &rstd});
   TORCH_CHECK(grad_output_.sizes() == input_.sizes() &&
                   grad_output_.scalar_type() == input_.scalar_type(),
               "bevk: grad_output must have input's shape and dtype");
@@ -209,7 +219,7 @@ int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.siz
 Tensor embedding_forward(const Tensor &table, const Tensor &ids_, double scale) {
   check_cuda(table, "weight");
   check_same_device(table, ids_, "ids");
-  check_no_tangent(table, "weight");
+  check_no_tangents({&table});
   TORCH_CHECK(table.dim() == 2 && table.size(1) > 0, "bevk: weight must be [rows, dim]");
   TORCH_CHECK(table.size(1) < (int64_t(1) << 24), "bevk: weight has too many columns");
   const bool wide = wide_ids(ids_);
@@ -232,7 +242,7 @@ Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t
                           double scale, int64_t padding_idx, const OptTensor &into) {
   check_cuda(grad_output, "grad_output");
   check_same_device(grad_output, ids_, "ids");
-  check_no_tangent(grad_output, "grad_output");
+  check_no_tangents({&grad_output, opt_ptr(into)});
   const bool wide = wide_ids(ids_);
   TORCH_CHECK(grad_output.dim() == ids_.dim() + 1 &&
                   grad_output.sizes().slice(0, ids_.dim()) == ids_.sizes(),
@@ -248,7 +258,6 @@ Tensor embedding_backward(const Tensor &grad_output, const Tensor &ids_, int64_t
   Tensor out;
   if (into) {
     check_same_device(grad_output, *into, "grad_weight");
-    check_no_tangent(*into, "grad_weight");
     TORCH_CHECK(into->dim() == 2 && into->size(0) == num_rows && into->size(1) == dim,
                 "bevk: grad_weight must be [num_embeddings, dim]");
     TORCH_CHECK((dim == 1 || into->stride(1) == 1) &&
@@ -295,6 +304,11 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
   const at::NoGradGuard no_grad;  // the copies below are no part of the caller's graph
   TORCH_CHECK(!grads.empty(), "bevk: no gradients");
   TORCH_CHECK(!out || out->size() == grads.size(), "bevk: one output for each gradient");
+  if (tangents_possible()) {
+    for (const Tensor &t : grads) check_no_tangent(t);
+    if (max_norm && out)
+      for (const Tensor &t : *out) check_no_tangent(t);
+  }
   const Tensor &first = grads[0];
   std::vector<bevk_grad_tensor> items(grads.size());
   std::vector<Tensor> keep;                          // copies the call reads or writes
@@ -308,8 +322,6 @@ Tensor grad_clip(const std::vector<Tensor> &grads, std::optional<double> max_nor
       check_same_device(first, g, "gradient");
     }
     TORCH_CHECK(g.layout() == at::kStrided, "bevk: gradients must be strided tensors");
-    check_no_tangent(g, "gradient");
-    if (max_norm && out) check_no_tangent((*out)[i], "output");
     bevk_grad_tensor &it = items[i];
     it.grad_dtype = dtype_of(g);
     it.numel = g.numel();
