@@ -25,7 +25,7 @@
 // Device time: 65536 rows of 4 KB looked up in 61 us (333 MB, 5.4 TB/s); their
 // gradient added to 10000 fp32 rows in 130 us (430 MB; the sort 20 us of it);
 // 16384 tokens into a dense 50021 x 1024 bf16 table in 41 us (136 MB); 40000
-// tokens of 200 rows of 512 bytes in 19 us, of which the sort is 9; 30 tokens in
+// tokens of 200 rows of 512 bytes in 17 us, of which the sort is 9; 30 tokens in
 // 12 us, the launches of zeros, sort and sums.
 #include <cuda_runtime.h>
 
@@ -784,7 +784,8 @@ int most_sorting_ctas() {
 
 // One CTA takes up to 2048 tokens (8.2 us for two passes of 2000; two CTAs 8.7,
 // but four CTAs 9.0 and one 12.7 for 4000), then a token a thread up to the
-// largest cluster, then 2, 4 or 8 a thread in registers, then any number.
+// largest cluster, then 2, 4 or 8 a thread in registers (8 spill 48 bytes), then any
+// number.
 constexpr int kOneCta = 2 * kSortThreads;
 template <typename Id>
 int sort_any(const SortParams &p, cudaStream_t stream) {

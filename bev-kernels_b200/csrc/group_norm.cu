@@ -36,15 +36,20 @@
 // single values are far out.
 //
 // Device time, forward / backward (inputs in L2 where they fit; 16-bit unless
-// said; bytes are the 2 and 3 passes): 1x64x32x32 fp32 ReLU 6.4 us; 6x512x29x50
-// ReLU 9.8 (1.8 TB/s) / 16.8; 6x256x58x100 SiLU 14.2 / 28 us (2.5 / 1.9 TB/s);
-// 1x256x200x200 fp32 SiLU 19.7 / 45 us (4.2 / 2.7); 12x256x116x200 SiLU 94 / 174 us
-// (3.0 / 2.5).  The small ones are the latency of launch, load, reduction, meeting
-// and store, about 1 to 1.5 us each.  Where all images are one wave the sweeps are
-// reads alone and then writes alone, and writes alone reach 3.3 to 3.9 TB/s on
-// this part.  Later waves mix the two; there a meeting waits for the stores of
-// the wave before (2 to 3 us).  Without an activation the large backward takes
-// 139 us: SiLU's instructions, in both of its sweeps, are the rest.
+// said; bytes are the 2 and 3 passes): 1x64x32x32 fp32 ReLU 6.4 / 8.3 us; 6x512x29x50
+// ReLU 9.8 (1.8 TB/s) / 14.8; 6x256x58x100 SiLU 14.1 / 26.3 us (2.5 / 2.0 TB/s);
+// 1x256x200x200 fp32 SiLU 17.3 / 43 us (4.7 / 2.9); 12x256x116x200 SiLU 91 / 174 us
+// (3.1 / 2.5).  The small ones are the latency of launch, load, reduction, meeting
+// and store, about 1 to 1.5 us each.  Of a wave of the largest, 22 % (backward) and
+// 23 % (forward) go to partial results, meeting and join, in which nothing moves:
+// there is one CTA an SM, and all go through the steps together.  The second sweep,
+// 57 % of a forward wave, writes, and fetches the next wave, at 4.9 TB/s together.
+// Without an activation the large backward takes 136 us: SiLU's instructions, in
+// both of its sweeps, are the rest.
+//
+// A wave has an image per CTA at most, so many small images are many waves: 1000 x
+// 256 x 7 x 7 bf16 take 36 / 39 us (floor 8 / 12), 20000 x 256 single pixels, one of
+// 16 rows of threads at work, 567 / 449 us (3 / 5).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -61,7 +66,9 @@ namespace bevk {
 namespace {
 
 // Threads of a CTA.  More of them leave each too few registers: 1024 (forward)
-// and 768 (backward) measured 1.2 to 1.5 times the time, with spills.
+// and 768 (backward) measured 1.2 to 1.5 times the time, with spills.  With 512 the
+// 16-bit backward spills 12 bytes with SiLU, and 80 to 204 where vectors cross groups
+// (6x264x58x100 bf16 SiLU of 24 groups 33.2 us, of 256 channels in 32 groups 25.8).
 constexpr int kForwardThreads = 512;
 constexpr int kBackwardThreads = 512;
 constexpr int kBatch = 8;  // vectors of one asynchronous group, or loaded directly
@@ -921,8 +928,15 @@ int most_slabs(const GnParams &p) {
 // channel block).  A wave is as many images as make twice what the CTAs hold, at
 // least one; the waves are then made equal.  What is not held is read twice, the
 // second time from L2; against waves that are held whole, fewer meetings of the
-// grid gain more: 12x256x116x200 bf16 backward 193 -> 174 us, 6x256x58x100 33 ->
-// 28 us (three times as much: 177, and the forward loses a sixth).
+// grid gain more, and three times as much gains and loses.  SiLU, forward /
+// backward in us with once, twice, three times what is held:
+//   12x256x116x200 bf16    91 / 197    91 / 174   108 / 176
+//   12x256x116x200 fp32   164 / 274   167 / 273   201 / 273
+//   7x256x116x200 bf16     63 / 118    60 / 118    66 / 127
+//   13x256x58x100 bf16     29 / 69     22 / 56     22 / 50
+//   6x256x58x100 fp32      20 / 40     16 / 36     16 / 33
+//   4x256x200x200 fp32     93 / 175    93 / 175   114 / 175
+// (one image is one wave: 1x256x400x400 bf16 65 / 109, 1x256x300x300 fp32 69 / 106).
 int set_slabs(GnParams *p, int ctas, int room) {
   const int64_t image = (p->HW + p->R - 1) / p->R;  // vectors of a thread for a whole image
   const int64_t most = std::max<int64_t>(
@@ -963,7 +977,8 @@ size_t gpart_bytes(const GnParams &p) {
 // little to do: measured against the grid (device time), 64x32x32 f32 6.4 and
 // 7.4 us, 30x128x28x28 bf16 10.6 and 11.6, 6x512x29x50 f16 (12 vectors a thread)
 // 9.8 and 9.9, but 1x256x58x100 bf16 (24 vectors) 15.7 and 9.1.
-// Sets the slabs and returns true where it is used.
+// Sets the slabs and returns true where it is used.  (The forward's alone: the backward
+// ends in channel sums over all CTAs, behind a meeting of the grid.)
 constexpr int kMostHeldByCluster = 12;
 template <auto kernel>
 bool set_clusters(GnParams *p, int room) {
